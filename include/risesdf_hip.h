@@ -51,6 +51,7 @@ const char *rsdf_last_error(void);
 #define RSDF_STATUS_X2_BWD_GUARDED 2   /* rsdf_sdfmlp_fd7_bwd_x2 launches that the range guard examined */
 #define RSDF_STATUS_PAIR_PACK_NONFINITE 3 /* of word 0's count: waves of rsdf_pair_pack / _pack2 (a network INPUT out of range) */
 #define RSDF_STATUS_PAIR_FWD_NONFINITE 4  /* of word 0's count: workgroups of rsdf_pair_fwd (a weight or hidden activation) */
+#define RSDF_STATUS_BAD_IDS 5             /* rows whose id / label / listed class lies outside its table (rsdf_embedding_fwd, rsdf_class_head_fwd) */
 
 /* ---- M1: ray/AABB slab test ----------------------------------------------------------------
  * replaces _C.ray_aabb_intersect  (lib/nerfacc/cuda/csrc/intersection.cu:93-133, pybind.cu) and
@@ -702,6 +703,46 @@ int rsdf_loss_samples_fwd(const float *sdf, const float *sdf_grad, const float *
 int rsdf_loss_samples_bwd(const float *sdf, const float *sdf_grad, const float *laplace, float sparsity_scale,
                           const float *coef3, int64_t n, float *d_sdf, float *d_sdf_grad, float *d_laplace,
                           void *stream);
+
+/* ---- code lookup by id (beside the hash grid's lookup by position) --------------------------------------------
+ * out[n][:] = scale * table[ids[n]][:] for ids [n], table [v][d], out [n][d]; dtype 0 fp32, 1 bf16, 2 fp16 (fp32 products, one
+ * rounding).  ids[n] == padding_id (INT64_MIN: none): a zero row; outside [0, v): a row of NaN, counted into *bad_ids
+ * (nullable, accumulates).
+ * bwd: d_table[v][:] = scale * sum of grad[n][:] over ids[n] == v, every row written (zero without a position; padding and
+ * outside ids take no part); no float atomics: results repeat bit for bit.
+ * workspace: >= rsdf_embedding_bwd_workspace_bytes(n, v, d) bytes. */
+int rsdf_embedding_fwd(const int64_t *ids, int64_t n, const void *table, int64_t v, int d, int dtype, float scale,
+                       int64_t padding_id, void *out, int32_t *bad_ids, void *stream);
+int64_t rsdf_embedding_bwd_workspace_bytes(int64_t n, int64_t v, int d);
+int rsdf_embedding_bwd(const int64_t *ids, int64_t n, const void *grad, int64_t v, int d, int dtype, float scale,
+                       int64_t padding_id, void *d_table, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* ---- losses of a linear head over many classes, without the logits in memory ------------------------------------
+ * z = x w^T for x [n][d], w [v][d] (both of `dtype`: 0 fp32, 1 bf16, 2 fp16; 16-byte aligned).  fp32 is computed with three-part
+ * split products (fp32-equivalent for finite operands; an infinite one makes NaN).
+ *   labels    teacher_logits NULL, k = 1: ids [n]; loss_n = lse_n - z[n][ids[n]]; a row with ids[n] == ignore_id takes part in
+ *             nothing.  temperature 1.
+ *   teacher   ids [n][k], teacher_logits [n][k] (the teacher's top logits): entries with id < 0 are absent whatever their logit
+ *             holds; q = softmax of the others / temperature; loss_n = temperature^2 sum_k q_k (log q_k - log softmax(z /
+ *             temperature)[ids_k]).  A row without an entry (or with logits of -inf only) takes part in nothing.
+ * Rows that take part in nothing have loss 0 and zero gradients and add nothing to dw, whatever x holds there.  A label or
+ * listed id outside [0, v) makes its row's loss NaN, adds nothing to the gradients and is counted into *bad_ids (nullable,
+ * accumulates).
+ * fwd: reduction 0: loss [n]; 1: loss [1] = mean over the rows that take part (0 without any), count [1] = their number (at
+ *   least 1); 2: loss [1] = sum.  lse [n], q [n][k] and listed_z [n][k] (teacher only) are what bwd reads.
+ * bwd: grad = d(loss): [n] (grad_per_row) or [1]; count as written by fwd for reduction 1, else NULL.  dx [n][d] / dw [v][d]
+ *   (nullable: not computed).
+ * workspace: >= rsdf_class_head_workspace_bytes(n, v, d, dtype, pass), pass 0 forward, else backward (1 dx, 2 dw, 3 both);
+ * its size does not grow with n * v. */
+int64_t rsdf_class_head_workspace_bytes(int64_t n, int64_t v, int d, int dtype, int pass);
+int rsdf_class_head_fwd(const void *x, const void *w, int64_t n, int64_t v, int d, int dtype, const int64_t *ids,
+                        const float *teacher_logits /*nullable*/, int k, int64_t ignore_id, float temperature, int reduction,
+                        float *loss, float *lse, float *count, float *q, float *listed_z, int32_t *bad_ids,
+                        void *workspace, int64_t workspace_bytes, void *stream);
+int rsdf_class_head_bwd(const void *x, const void *w, int64_t n, int64_t v, int d, int dtype, const int64_t *ids,
+                        const float *q /*nullable*/, const float *listed_z /*nullable*/, int k, float temperature,
+                        const float *lse, const float *count /*nullable*/, const float *grad, int grad_per_row, void *dx,
+                        void *dw, void *workspace, int64_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

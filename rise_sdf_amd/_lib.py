@@ -164,6 +164,12 @@ _SIGNATURES = {
     "rsdf_neus_alpha_fwd": [_P, _P, _P, _P, _P, _F, _L, _P, _P],
     "rsdf_neus_alpha_bwd": [_P, _P, _P, _P, _P, _F, _L, _P, _P, _P, _P, _P],
     "rsdf_neus_occ_alpha": [_P, _P, _F, _L, _P, _P],
+    "rsdf_embedding_fwd": [_P, _L, _P, _L, _I, _I, _F, _L, _P, _P, _P],
+    "rsdf_embedding_bwd_workspace_bytes": [_L, _L, _I],
+    "rsdf_embedding_bwd": [_P, _L, _P, _L, _I, _I, _F, _L, _P, _P, _L, _P],
+    "rsdf_class_head_workspace_bytes": [_L, _L, _I, _I, _I],
+    "rsdf_class_head_fwd": [_P, _P, _L, _L, _I, _I, _P, _P, _I, _L, _F, _I, _P, _P, _P, _P, _P, _P, _P, _L, _P],
+    "rsdf_class_head_bwd": [_P, _P, _L, _L, _I, _I, _P, _P, _P, _I, _F, _P, _P, _P, _I, _P, _P, _P, _L, _P],
 }
 # config[4]'s bf16 MLP mode: the MLP entry points a second time with the suffix _bf16 (same signatures; split_bf16.h)
 BF16_ENTRY_POINTS = ("rsdf_linear_fwd", "rsdf_linear_bwd_input", "rsdf_linear_bwd_weight",
@@ -187,7 +193,8 @@ def mlp_fn(name, precision="fp32"):
     raise ValueError(f"unknown MLP precision {precision!r} (fp32, bf16 or fp16)")
 
 
-_RESTYPES = {"rsdf_last_error": ctypes.c_char_p, "rsdf_scan_scratch_bytes": ctypes.c_int64,
+_RESTYPES = {"rsdf_last_error": ctypes.c_char_p, "rsdf_embedding_bwd_workspace_bytes": ctypes.c_int64,
+             "rsdf_class_head_workspace_bytes": ctypes.c_int64, "rsdf_scan_scratch_bytes": ctypes.c_int64,
              "rsdf_x2_rows": ctypes.c_int64, "rsdf_x2_bytes": ctypes.c_int64, "rsdf_pair_image_bytes": ctypes.c_int64,
              "rsdf_grid_meta_init": ctypes.c_int64,
              "rsdf_hashgrid_bwd_fd7_scratch_bytes": ctypes.c_int64,
@@ -258,7 +265,7 @@ class _TimedLib:
     def __getattr__(self, name):
         fn = getattr(self._l, name)
         # host-only queries launch nothing: not timed
-        if not name.startswith("rsdf_") or "_supported" in name or name.endswith("_scratch_bytes") or \
+        if not name.startswith("rsdf_") or "_supported" in name or name.endswith(("_scratch_bytes", "_workspace_bytes")) or \
                 name in ("rsdf_last_error", "rsdf_abi_version", "rsdf_grid_meta_init"):
             return fn
         timer = self._t
@@ -418,9 +425,11 @@ def free_workspaces():
 # two sampler counts): ``poll_status`` right behind such a read costs one more 32-byte copy on an already drained stream.
 STATUS_WORDS = 8
 ST_X2_FWD_NONFINITE, ST_X2_BWD_REROUTED, ST_X2_BWD_GUARDED, ST_PAIR_PACK_NONFINITE, ST_PAIR_FWD_NONFINITE = 0, 1, 2, 3, 4
+ST_BAD_IDS = 5
 _STATUS = {}
 _STATUS_SEEN = {}        # device index -> the raw words at the last poll (the device-side words are MONOTONIC: never cleared)
-_STATUS_TOTALS = {"x2_bwd_rerouted": 0, "x2_bwd_guarded": 0, "x2_fwd_nonfinite_total": 0, "range_reroutes": 0}
+_STATUS_TOTALS = {"x2_bwd_rerouted": 0, "x2_bwd_guarded": 0, "x2_fwd_nonfinite_total": 0, "range_reroutes": 0,
+                  "bad_ids": 0}
 
 # What a forward range violation of the two-part fp16 kernels does (the reference's fp32 MLPs have no such limit and simply
 # continue, models/network_utils.py:109-157):
@@ -459,6 +468,16 @@ def status(device) -> "torch.Tensor":
     return t
 
 
+def bad_ids_ptr(device):
+    """Where kernels count ids outside their table (status word ST_BAD_IDS).  None while a graph is being captured on a device
+    that has no status words yet: they would live in the graph's private pool."""
+    dev = torch.device(device)
+    idx = dev.index if dev.index is not None else torch.cuda.current_device()
+    if idx not in _STATUS and torch.cuda.is_current_stream_capturing():
+        return None
+    return ptr(status(dev)[ST_BAD_IDS:])
+
+
 def _status_delta(idx, vals):
     """Counts since the last poll of device ``idx`` (wrap-around safe), and remember ``vals`` as seen."""
     seen = _STATUS_SEEN.setdefault(idx, [0] * STATUS_WORDS)
@@ -474,14 +493,15 @@ def poll_status(device=None, raise_on_error=True) -> dict:
     family to the range-free kernels (``range_policy``; RSDF_RANGE_ERROR=raise: RiseSdfHipError instead)."""
     keys = list(_STATUS) if device is None else [torch.device(device).index if torch.device(device).index is not None
                                                  else torch.cuda.current_device()]
-    bad, sites, rerouted = 0, [0, 0], False
+    bad, sites, ids = 0, [0, 0], 0
     for idx in keys:
         t = _STATUS.get(idx)
         if t is not None:
             r = consume_status(t, t.tolist(), raise_on_error=False, _defer=True)
             bad += r["x2_fwd_nonfinite"]
             sites = [a + b for a, b in zip(sites, r["_sites"])]
-    return _status_result(bad, raise_on_error, sites)
+            ids += r["_bad_ids"]
+    return _status_result(bad, raise_on_error, sites, ids)
 
 
 def consume_status(t, vals, raise_on_error=True, _defer=False) -> dict:
@@ -492,8 +512,8 @@ def consume_status(t, vals, raise_on_error=True, _defer=False) -> dict:
     _STATUS_TOTALS["x2_bwd_guarded"] += d[ST_X2_BWD_GUARDED]
     sites = d[ST_PAIR_PACK_NONFINITE:ST_PAIR_FWD_NONFINITE + 1]
     if _defer:
-        return {"x2_fwd_nonfinite": d[ST_X2_FWD_NONFINITE], "_sites": sites}
-    return _status_result(d[ST_X2_FWD_NONFINITE], raise_on_error, sites)
+        return {"x2_fwd_nonfinite": d[ST_X2_FWD_NONFINITE], "_sites": sites, "_bad_ids": d[ST_BAD_IDS]}
+    return _status_result(d[ST_X2_FWD_NONFINITE], raise_on_error, sites, d[ST_BAD_IDS])
 
 
 def _range_message(bad, sites):
@@ -506,8 +526,9 @@ def _range_message(bad, sites):
             "|input|, |weight| or a hidden activation >= 1023 -- where the reference's fp32 MLPs stay finite.")
 
 
-def _status_result(bad, raise_on_error, sites=(0, 0)):
+def _status_result(bad, raise_on_error, sites=(0, 0), ids=0):
     rerouted = False
+    _STATUS_TOTALS["bad_ids"] += ids
     if bad:
         _STATUS_TOTALS["x2_fwd_nonfinite_total"] += bad
         if raise_on_error and range_policy() == "raise":
@@ -528,6 +549,10 @@ def _status_result(bad, raise_on_error, sites=(0, 0)):
                     "call that overflowed is recomputed where its caller still holds the inputs (samplers, "
                     "rise_sdf_amd.guarded, TrainStep skips that optimizer step).  RSDF_RANGE_ERROR=raise raises instead.",
                     RuntimeWarning, stacklevel=3)
+    if ids and raise_on_error:
+        raise RiseSdfHipError(f"{ids} rows named an id outside the table (ops.embedding) or a label / listed class outside the "
+                              "head (loss.linear_cross_entropy, loss.linear_distillation) since the last check: their "
+                              "outputs are NaN and they took no part in the gradients")
     return dict(_STATUS_TOTALS, x2_fwd_nonfinite=bad, rerouted_now=rerouted)
 
 

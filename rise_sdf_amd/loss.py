@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import torch
 
+from . import _lib as L
 from ._lib import check, lib, ptr, require_device, stream_ptr
 
 
@@ -117,3 +118,130 @@ def loss_tail(out, batch, lambdas, sparsity_scale=1.0, has_mask=True):
                                    out["sdf_grad_samples"], lap, batch["rgb"], out["rays_valid_full"],
                                    batch.get("fg_mask", None), tuple(lam), float(sparsity_scale))
     return total, {"loss_" + k: terms[i].detach() for i, k in enumerate(TERMS)}
+
+
+# ------------------------------------------------------------------------------------------------
+# losses of a linear head over many classes (csrc/class_head.hip): the logits are never stored
+# ------------------------------------------------------------------------------------------------
+_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+
+
+def _aligned(t):
+    """Contiguous and 16-byte aligned (a view into the middle of a storage may be neither)."""
+    t = t.detach().contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+class _ClassHead(torch.autograd.Function):
+    """Both losses: ``logits`` None = labels (``ids`` [N, 1]), else a teacher's listed classes (``ids``, ``logits`` [N, K])."""
+
+    @staticmethod
+    def forward(ctx, x, w, ids, logits, ignore, temperature, reduction):
+        from .ops import DTYPE_IDS
+        xc, wc = _aligned(x), _aligned(w)
+        require_device(xc, wc, ids, logits)
+        dev, (n, d), v, k = xc.device, xc.shape, wc.shape[0], ids.shape[1]
+        dt = DTYPE_IDS[xc.dtype]
+        with torch.cuda.device(dev):
+            def f32(*shape):
+                return torch.empty(shape, dtype=torch.float32, device=dev)
+            nbytes = int(lib().rsdf_class_head_workspace_bytes(n, v, d, dt, 0))
+            if nbytes < 0:
+                check(1, "class_head_workspace_bytes")
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            loss, lse = f32(n) if reduction == 0 else f32(1), f32(n)
+            count = f32(1) if reduction else None
+            q, zt = (f32(n, k), f32(n, k)) if logits is not None else (None, None)
+            check(lib().rsdf_class_head_fwd(ptr(xc), ptr(wc), n, v, d, dt, ptr(ids), ptr(logits), k, ignore, temperature,
+                                            reduction, ptr(loss), ptr(lse), ptr(count), ptr(q), ptr(zt),
+                                            L.bad_ids_ptr(dev), ptr(ws), nbytes, stream_ptr()), "class_head_fwd")
+        ctx.save_for_backward(xc, wc, ids, q, zt, lse, count)
+        ctx.temperature, ctx.reduction = temperature, reduction
+        return loss if reduction == 0 else loss.reshape(())
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        from .ops import DTYPE_IDS
+        xc, wc, ids, q, zt, lse, count = ctx.saved_tensors
+        need_x, need_w = ctx.needs_input_grad[:2]
+        if not (need_x or need_w):
+            return (None,) * 7
+        dev, (n, d), v, k = xc.device, xc.shape, wc.shape[0], ids.shape[1]
+        dt = DTYPE_IDS[xc.dtype]
+        g = g.detach().to(torch.float32).reshape(-1).contiguous()
+        with torch.cuda.device(dev):
+            dx = torch.empty_like(xc) if need_x else None
+            dw = torch.empty_like(wc) if need_w else None
+            nbytes = int(lib().rsdf_class_head_workspace_bytes(n, v, d, dt, int(need_x) + 2 * int(need_w)))
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            check(lib().rsdf_class_head_bwd(ptr(xc), ptr(wc), n, v, d, dt, ptr(ids), ptr(q), ptr(zt), k, ctx.temperature,
+                                            ptr(lse), ptr(count) if ctx.reduction == 1 else None, ptr(g),
+                                            int(ctx.reduction == 0), ptr(dx), ptr(dw), ptr(ws), nbytes, stream_ptr()),
+                  "class_head_bwd")
+        return dx, dw, None, None, None, None, None
+
+
+def _class_head(what, x, weight, ids, logits, ignore, temperature, reduction):
+    from .ops import _dtype_id, _int_ids, _same_device
+    err = L.RiseSdfHipError
+    if reduction not in _REDUCTIONS:
+        raise err(f"{what}: reduction {reduction!r}: none, mean or sum")
+    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
+        raise err(f"{what}: features [..., D] and class codes [V, D], not {tuple(x.shape)} and {tuple(weight.shape)}")
+    if weight.shape[0] < 1 or weight.shape[1] < 1:
+        raise err(f"{what}: the head needs at least one class and one feature")
+    if x.dtype != weight.dtype:
+        raise err(f"{what}: features and class codes of one type, not {x.dtype} and {weight.dtype}")
+    _dtype_id(x, what)
+    ids = _int_ids(ids, what)
+    tensors = (x, weight, ids) if logits is None else (x, weight, ids, logits)
+    _same_device(what, *tensors)
+    require_device(*(t.contiguous() for t in tensors))
+    lead = x.shape[:-1]
+    n = x.numel() // x.shape[-1]
+    if n == 0:                        # no rows: an empty, or zero, loss that still reaches its inputs' graph
+        zero = x.sum().float() * 0.0 + weight.reshape(-1)[:1].sum().float() * 0.0
+        return zero.expand(0).reshape(lead) if reduction == "none" else torch.nan_to_num(zero)
+    k = 1 if logits is None else ids.shape[-1]
+    out = _ClassHead.apply(x.reshape(n, x.shape[-1]), weight, ids.reshape(n, k),
+                           None if logits is None else _f(logits).reshape(n, k), int(ignore), float(temperature),
+                           _REDUCTIONS[reduction])
+    return out.reshape(lead) if reduction == "none" else out
+
+
+def linear_cross_entropy(x, weight, target, *, ignore_index=-100, reduction="mean"):
+    """Softmax cross entropy of the logits ``x @ weight.T`` against ``target``, without storing the logits (nor, in the
+    backward, more than a bounded piece of their gradient): per-ray features against a codebook of labels.
+
+    ``x`` [..., D], ``weight`` [V, D] of one type (fp32: fp32-equivalent split products; bf16 / fp16: fp32 sums), ``target``
+    [...] integers.  ``reduction``: "none" -> [...], "mean" over the rows that are not ignored (0 if all are), "sum"; fp32.
+    Differentiable w.r.t. ``x`` and ``weight`` (once).  Rows with ``target == ignore_index`` take part in nothing, whatever
+    ``x`` holds there; any other target outside [0, V) makes its row NaN, takes no part in the gradients and is reported by
+    ``rise_sdf_amd.check_status()``."""
+    if tuple(target.shape) != tuple(x.shape[:-1]):
+        raise L.RiseSdfHipError(f"linear_cross_entropy: one target per row: {tuple(target.shape)} for features "
+                                f"{tuple(x.shape)}")
+    return _class_head("linear_cross_entropy", x, weight, target, None, ignore_index, 1.0, reduction)
+
+
+def linear_distillation(x, weight, teacher_ids, teacher_logits, *, temperature=1.0, reduction="mean"):
+    """Distillation of a linear head from the top logits of a teacher, without storing the head's logits.
+
+    Per row: ``T^2 * sum_k q_k (log q_k - log_softmax(x @ weight.T / T)[ids_k])`` with ``q = softmax(teacher_logits / T)`` over
+    the listed classes: the divergence from the teacher's renormalised top classes.  ``x`` [..., D], ``weight`` [V, D] of one
+    type, ``teacher_ids`` [..., K] integers (negative: no entry, whatever its logit holds; a class may be listed twice),
+    ``teacher_logits`` [..., K] (no gradient).  Rows without an entry take part in nothing.  ``reduction``: "none" -> [...],
+    "mean" over the rows with an entry (0 if there are none), "sum"; fp32.  Differentiable w.r.t. ``x`` and ``weight`` (once).
+    A listed class >= V makes its row NaN, takes no part in the gradients and is reported by
+    ``rise_sdf_amd.check_status()``."""
+    if teacher_ids.shape != teacher_logits.shape or teacher_ids.shape[:-1] != x.shape[:-1]:
+        raise L.RiseSdfHipError(f"linear_distillation: ids and logits [..., K] per row: {tuple(teacher_ids.shape)} and "
+                                f"{tuple(teacher_logits.shape)} for features {tuple(x.shape)}")
+    if not 1 <= teacher_ids.shape[-1] <= 4096:
+        raise L.RiseSdfHipError("linear_distillation: between 1 and 4096 listed classes per row")
+    if not teacher_logits.dtype.is_floating_point:
+        raise L.RiseSdfHipError(f"linear_distillation: floating point logits, not {teacher_logits.dtype}")
+    if not 0.0 < float(temperature) < float("inf"):
+        raise L.RiseSdfHipError(f"linear_distillation: temperature {temperature} is not positive and finite")
+    return _class_head("linear_distillation", x, weight, teacher_ids, teacher_logits, -1, temperature, reduction)

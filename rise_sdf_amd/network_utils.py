@@ -5,6 +5,7 @@ and state_dict names), computing through the HIP ops.
   CompositeEncoding         models/network_utils.py:71-88
   VanillaMLP                models/network_utils.py:109-157
   get_encoding / get_mlp    models/network_utils.py:91-106, 194-204
+  EmbeddingEncoding         (no counterpart: codes by integer id)
 """
 from __future__ import annotations
 
@@ -92,8 +93,32 @@ class CompositeEncoding(nn.Module):
         return self.encoding.regularizations() if hasattr(self.encoding, "regularizations") else {}
 
 
+class EmbeddingEncoding(nn.Module):
+    """``otype: Embedding``: one learned code per integer id (a view, a material, a label) instead of a code per position:
+    ids [...] -> ``scale * params[ids]`` [..., n_features].  ``padding_idx``: the id without a code (zero rows, no gradient).
+    The same table can be the ``weight`` of ``loss.linear_cross_entropy`` / ``linear_distillation`` (a tied codebook)."""
+
+    def __init__(self, in_channels, config):
+        super().__init__()
+        if in_channels != 1:
+            raise NotImplementedError("Embedding encodes one integer id per input")
+        self.n_input_dims = 1
+        self.n_output_dims = int(config["n_features"])
+        self.scale = float(config.get("scale", 1.0))
+        self.padding_idx = config.get("padding_idx", None)
+        self.params = nn.Parameter(torch.randn(int(config["n_embeddings"]), self.n_output_dims) * float(config.get("std", 0.01)))
+        if self.padding_idx is not None:
+            with torch.no_grad():
+                self.params[self.padding_idx].zero_()
+
+    def forward(self, ids):
+        return ops.embedding(ids, self.params, scale=self.scale, padding_idx=self.padding_idx)
+
+
 def get_encoding(n_input_dims, config):
-    """Input is expected in [0,1] (:91-106)."""
+    """Input is expected in [0,1] (:91-106); ids for an ``Embedding``."""
+    if config.otype == "Embedding":
+        return EmbeddingEncoding(n_input_dims, config_to_primitive(config))
     if config.otype == "ProgressiveBandHashGrid":
         encoding = ProgressiveBandHashGrid(n_input_dims, config_to_primitive(config))
     elif config.otype in ("HashGrid", "Grid"):

@@ -696,6 +696,83 @@ def hashgrid_encode(x, table, meta, n_active_levels=None, include_xyz=False, xyz
 
 
 # ------------------------------------------------------------------------------------------------
+# lookup by id
+# ------------------------------------------------------------------------------------------------
+DTYPE_IDS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_NO_PADDING = -(1 << 63)
+
+
+def _dtype_id(t, what):
+    try:
+        return DTYPE_IDS[t.dtype]
+    except KeyError:
+        raise L.RiseSdfHipError(f"{what}: float32, bfloat16 or float16, not {t.dtype}") from None
+
+
+def _same_device(what, *tensors):
+    dev = tensors[0].device
+    if any(t.device != dev for t in tensors):
+        raise L.RiseSdfHipError(f"{what}: tensors on different devices ({', '.join(str(t.device) for t in tensors)})")
+    return dev
+
+
+def _int_ids(ids, what):
+    if ids.dtype not in (torch.int64, torch.int32, torch.int16, torch.uint8):
+        raise L.RiseSdfHipError(f"{what}: integer ids, not {ids.dtype}")
+    return ids.detach().to(torch.int64).contiguous()
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ids, table, scale, padding):
+        tb = table.detach().contiguous()
+        dt = _dtype_id(tb, "embedding")
+        require_device(ids, tb)
+        dev = _same_device("embedding", ids, tb)
+        V, D = tb.shape
+        with torch.cuda.device(dev):
+            out = torch.empty(*ids.shape, D, dtype=tb.dtype, device=dev)
+            check(lib().rsdf_embedding_fwd(ptr(ids), ids.numel(), ptr(tb), V, D, dt, scale, padding, ptr(out),
+                                           L.bad_ids_ptr(dev), stream_ptr()), "embedding_fwd")
+        ctx.save_for_backward(ids)
+        ctx.shape, ctx.dtype, ctx.scale, ctx.padding = (V, D), tb.dtype, scale, padding
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gout):
+        (ids,) = ctx.saved_tensors
+        V, D = ctx.shape
+        g = gout.detach().to(ctx.dtype).contiguous()
+        n, dev = ids.numel(), ids.device
+        with torch.cuda.device(dev):
+            dt = torch.empty(V, D, dtype=ctx.dtype, device=dev)
+            nbytes = int(lib().rsdf_embedding_bwd_workspace_bytes(n, V, D))
+            ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
+            check(lib().rsdf_embedding_bwd(ptr(ids), n, ptr(g), V, D, DTYPE_IDS[ctx.dtype], ctx.scale, ctx.padding, ptr(dt),
+                                           ptr(ws), nbytes, stream_ptr()), "embedding_bwd")
+        return None, dt, None, None
+
+
+def embedding(ids, table, scale=1.0, padding_idx=None):
+    """Codes by id: ``ids`` (integers, any shape) -> [*ids.shape, D] = ``scale * table[ids]`` for ``table`` [V, D] in fp32, bf16
+    or fp16 (fp32 products, one rounding).  ``padding_idx``: the id whose rows are zero and take no gradient.
+
+    Differentiable w.r.t. ``table`` (a dense gradient, summed in fp32 by sorted ids: the same bits every time).  An id outside
+    [0, V) (negative ones too: they do not wrap) gives a row of NaN, takes no part in the gradient and is reported by
+    ``rise_sdf_amd.check_status()`` and by the samplers' own polls."""
+    if not torch.is_tensor(table) or table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1:
+        raise L.RiseSdfHipError("embedding: table must be [V, D] with V, D >= 1")
+    _dtype_id(table, "embedding")
+    pad = _NO_PADDING
+    if padding_idx is not None:
+        pad = int(padding_idx)
+        if not 0 <= pad < table.shape[0]:
+            raise L.RiseSdfHipError(f"embedding: padding_idx {pad} outside the table's {table.shape[0]} rows")
+    return _Embedding.apply(_int_ids(ids, "embedding"), table, float(scale), pad)
+
+
+# ------------------------------------------------------------------------------------------------
 # H3
 # ------------------------------------------------------------------------------------------------
 def _dw_db(N, K, has_bias, device):
