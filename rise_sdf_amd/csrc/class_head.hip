@@ -31,7 +31,8 @@ namespace {
 constexpr int T_F32 = 0, T_BF16 = 1, T_F16 = 2;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float F16_DZ = 4096.0f;
-constexpr int64_t DZ_BYTES = 256ll << 20;      // of one piece of dz
+constexpr int64_t DZ_BYTES = 128ll << 20;      // of one piece of dz
+constexpr int CUS = 256;                        // MI355X
 constexpr int64_t WPACK_BYTES = 128ll << 20;   // of the packed class codes of one piece
 
 __device__ __forceinline__ float bf2f(unsigned short u) { return __builtin_bit_cast(float, (unsigned)u << 16); }
@@ -115,7 +116,7 @@ struct HeadArgs {
     Operand w, x;                // base of the piece's first class / of row 0
     int64_t n, vc;               // rows, classes of the piece
     int nseg;
-    int64_t ksteps;
+    int64_t depth;               // K: a multiple of 64
     float c;                     // log2(e) / T
     int64_t tiles_n, tiles;
     // statistics
@@ -130,90 +131,123 @@ struct HeadArgs {
     int64_t n_pad, ldz;
 };
 
-template <class TL, bool DZ, int PARTS>
-__global__ void __launch_bounds__(THREADS, 2) head_kernel(HeadArgs a)
+// operands of tile t and where it lies
+template <class TL>
+__device__ __forceinline__ void head_tile(const HeadArgs &a, int64_t t, Operand &W, Operand &X, int64_t &m0, int64_t &n0)
 {
-    __shared__ __attribute__((aligned(1024))) unsigned char lds[TL::LDS];
-    const int64_t t = xcd_tile(a.tiles);
-    if (t < 0) return;
-    const int64_t tm = t / a.tiles_n, tn = t % a.tiles_n;
-    const int64_t m0 = tm * TL::BM, n0 = tn * TL::BN;
-    Operand W = a.w, X = a.x;
-    const bool rows_here = n0 < a.n;            // (dz: the tiles of padding rows only write zeros)
+    m0 = t / a.tiles_n * TL::BM;
+    n0 = t % a.tiles_n * TL::BN;
+    W = a.w;
+    X = a.x;
     W.base += m0 * W.ld;
     W.lim = (int)(a.vc - 1 - m0 < TL::BM - 1 ? a.vc - 1 - m0 : TL::BM - 1);
-    if (rows_here) X.base += n0 * X.ld;
-    X.lim = rows_here ? (int)(a.n - 1 - n0 < TL::BN - 1 ? a.n - 1 - n0 : TL::BN - 1) : 0;
-    f32x4 acc[TL::MT][TL::NT];
-#pragma unroll
-    for (int i = 0; i < TL::MT; ++i)
-#pragma unroll
-        for (int j = 0; j < TL::NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    TL::run(acc, W, X, a.nseg, a.ksteps, 0, rows_here ? a.nseg * a.ksteps : 0, lds);
+    X.base += n0 * X.ld;
+    X.lim = (int)(a.n - 1 - n0 < TL::BN - 1 ? a.n - 1 - n0 : TL::BN - 1);
+}
 
-    const int64_t left = a.vc - m0;         // valid classes of this tile
-    if (!DZ) {
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / TL::WN;
-        float2 *part = (float2 *)lds;           // [WM][BN]
+// per row: lse, the weight relative to the largest (0: the row takes part in nothing, whatever its logits are), the label's class
+// relative to the tile's first
+template <class TL>
+struct RowState {
+    float lse[TL::NT], f[TL::NT];
+    int label[TL::NT];
+    __device__ __forceinline__ void load(const HeadArgs &a, int64_t m0, int64_t n0)
+    {
+        const float top = a.top[0];
 #pragma unroll
         for (int nt = 0; nt < TL::NT; ++nt) {
-            float mx = -__builtin_inff();
+            const int64_t n = n0 + TL::n_of(nt);
+            lse[nt] = n < a.n ? a.lse[n] : __builtin_inff();
+            f[nt] = lse[nt] != __builtin_inff() ? a.weight[n] / top * (TL::F16 ? F16_DZ : 1.0f) : 0.0f;
+            const int64_t l = (f[nt] != 0.0f && a.label != nullptr) ? a.label[n] - a.v0 - m0 : -1;
+            label[nt] = l >= 0 && l < TL::BM ? (int)l : -1;
+            // here, and not behind the requests of the next tile: the loads' wait would wait for those too
+            asm volatile("" ::"v"(lse[nt]), "v"(f[nt]), "v"(label[nt]));
+        }
+    }
+};
+
+template <class TL, bool DZ, int PARTS>
+__device__ __forceinline__ void head_results(const HeadArgs &a, typename TL::Acc &acc, const RowState<TL> &rows, int64_t m0, int64_t n0,
+                                             float2 *part /* [WM][BN], LDS */)
+{
+    const bool whole = a.vc - m0 >= TL::BM;     // else the last classes of the tile are not there
+    const int left = whole ? TL::BM : (int)(a.vc - m0);
+    if (!DZ) {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / TL::WN;
+        if (!whole) {
 #pragma unroll
             for (int mt = 0; mt < TL::MT; ++mt) {
                 const int m = TL::m_of(mt >> 2) + (mt & 3) * 4;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    float z = acc[mt][nt][r] * a.c;
-                    z = m + r < left ? z : -__builtin_inff();
-                    acc[mt][nt][r] = z;
-                    mx = fmaxf(mx, z);
-                }
+                for (int nt = 0; nt < TL::NT; ++nt)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) acc[mt][nt][r] = m + r < left ? acc[mt][nt][r] : -__builtin_inff();
             }
-            mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-            const float ref = mx > -__builtin_inff() ? mx : 0.0f;
-            float s = 0.0f;
+        }
+#pragma unroll
+        for (int nt = 0; nt < TL::NT; ++nt) {
+            // (c > 0: the maximum of z is that of c z; one fma, one exponential and one sum per logit)
+            float mx = -__builtin_inff();
 #pragma unroll
             for (int mt = 0; mt < TL::MT; ++mt)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) s += __builtin_amdgcn_exp2f(acc[mt][nt][r] - ref);
-            s += __shfl_xor(s, 16, 64);
-            s += __shfl_xor(s, 32, 64);
-            if (lane < 16) part[wm * TL::BN + TL::n_of(nt)] = float2{mx, s};
+                for (int r = 0; r < 4; ++r) mx = fmaxf(mx, acc[mt][nt][r]);
+            mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            mx *= a.c;
+            const float ref = mx > -__builtin_inff() ? mx : 0.0f;
+            float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int mt = 0; mt < TL::MT; ++mt)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[r] += __builtin_amdgcn_exp2f(fmaf(acc[mt][nt][r], a.c, -ref));
+            float t = (s[0] + s[1]) + (s[2] + s[3]);
+            t += __shfl_xor(t, 16, 64);
+            t += __shfl_xor(t, 32, 64);
+            if (lane < 16) part[wm * TL::BN + TL::n_of(nt)] = float2{mx, t};
         }
         __syncthreads();
-        for (int n = threadIdx.x; n < TL::BN; n += THREADS) {
+        for (int n = threadIdx.x; n < TL::BN; n += TL::THREADS) {
             if (n0 + n >= a.n) continue;
             float2 p = part[n];
 #pragma unroll
             for (int k = 1; k < TL::WM; ++k) p = join_stats(p, part[k * TL::BN + n]);
-            a.stats[(a.tile0 + tm) * a.n + n0 + n] = p;
+            a.stats[(a.tile0 + m0 / TL::BM) * a.n + n0 + n] = p;
         }
     } else {
         constexpr bool F16 = TL::F16;
 #pragma unroll
         for (int nt = 0; nt < TL::NT; ++nt) {
             const int64_t n = n0 + TL::n_of(nt);
-            const float lse = n < a.n ? a.lse[n] : __builtin_inff();
-            const bool live = lse != __builtin_inff();
-            const float f = live ? a.weight[n] / a.top[0] * (F16 ? F16_DZ : 1.0f) : 0.0f;
-            const int64_t label = (live && a.label != nullptr) ? a.label[n] - a.v0 - m0 : -1;
+            const float lse = rows.lse[nt], f = rows.f[nt];
+            const int label = rows.label[nt];
 #pragma unroll
             for (int b = 0; b < TL::MT / 4; ++b) {
                 const int m = TL::m_of(b);
+                float p[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(acc[4 * b + (e >> 2)][nt][e & 3], a.c, -lse));
+                if (label >= m && label < m + 16) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) p[e] -= m + e == label ? 1.0f : 0.0f;
+                }
+#pragma unroll
+                for (int e = 0; e < 16; ++e) p[e] *= f;
+                if (f == 0.0f || !whole) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) p[e] = f != 0.0f && m + e < left ? p[e] : 0.0f;
+                }
                 unsigned short o[PARTS][16];
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    float p = __builtin_amdgcn_exp2f(acc[4 * b + (e >> 2)][nt][e & 3] * a.c - lse);
-                    p = m + e == label ? p - 1.0f : p;
-                    p = f != 0.0f && m + e < left ? p * f : 0.0f;
                     if (PARTS == 3) {
                         unsigned short h[3];
-                        split3(p, h);
+                        split3(p[e], h);
 #pragma unroll
                         for (int k = 0; k < PARTS; ++k) o[k][e] = h[k];
                     } else {
-                        o[0][e] = to16<F16>(p);
+                        o[0][e] = to16<F16>(p[e]);
                     }
                 }
 #pragma unroll
@@ -224,6 +258,69 @@ __global__ void __launch_bounds__(THREADS, 2) head_kernel(HeadArgs a)
                 }
             }
         }
+    }
+}
+
+template <class TL>
+__device__ __forceinline__ void clear(typename TL::Acc &acc)
+{
+#pragma unroll
+    for (int i = 0; i < TL::MT; ++i)
+#pragma unroll
+        for (int j = 0; j < TL::NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+}
+
+// few rows: one tile per workgroup
+template <class TL, bool DZ, int PARTS>
+__global__ void __launch_bounds__(TL::THREADS, TL::OCCUPANCY) head_kernel(HeadArgs a)
+{
+    __shared__ __attribute__((aligned(1024))) unsigned char lds[TL::LDS];
+    const int64_t t = xcd_tile(a.tiles);
+    if (t < 0) return;
+    Operand W, X;
+    int64_t m0, n0;
+    head_tile<TL>(a, t, W, X, m0, n0);
+    typename TL::Acc acc;
+    clear<TL>(acc);
+    const int64_t ksteps = a.depth / TL::KD;
+    TL::run(acc, W, X, a.nseg, ksteps, 0, a.nseg * ksteps, lds);
+    RowState<TL> rows;
+    if (DZ) rows.load(a, m0, n0);
+    head_results<TL, DZ, PARTS>(a, acc, rows, m0, n0, (float2 *)lds);
+}
+
+// One workgroup per CU walks its tiles; the first steps of the next tile are on their way while the results of this one are
+// worked out.  Each XCD has a contiguous eighth of the tiles (rows run fastest) and its workgroups take neighbouring ones:
+// they share the class codes in the XCD's L2.
+template <class TL, bool DZ, int PARTS>
+__global__ void __launch_bounds__(TL::THREADS, TL::OCCUPANCY) head_walk_kernel(HeadArgs a)
+{
+    __shared__ __attribute__((aligned(1024))) unsigned char lds[TL::LDS];
+    __shared__ float2 part[TL::WM * TL::BN];
+    const int64_t per = (a.tiles + 7) / 8, first = (blockIdx.x & 7) * per, stride = gridDim.x >> 3;
+    const int64_t end = first + per < a.tiles ? first + per : a.tiles;
+    const int64_t ksteps = a.depth / TL::KD, steps = a.nseg * ksteps;
+    int64_t t = first + (blockIdx.x >> 3);
+    if (t >= end) return;
+    Operand W, X;
+    int64_t m0, n0;
+    typename TL::Pipe pipe;
+    head_tile<TL>(a, t, W, X, m0, n0);
+    pipe.begin(W, X, a.nseg, ksteps, 0, steps, lds);
+    for (;;) {
+        typename TL::Acc acc;
+        clear<TL>(acc);
+        pipe.finish(acc);
+        RowState<TL> rows;
+        if (DZ) rows.load(a, m0, n0);
+        const int64_t m = m0, n = n0;
+        t += stride;
+        if (t < end) {
+            head_tile<TL>(a, t, W, X, m0, n0);
+            pipe.begin(W, X, a.nseg, ksteps, 0, steps, lds);
+        }
+        head_results<TL, DZ, PARTS>(a, acc, rows, m, n, part);
+        if (t >= end) return;
     }
 }
 
@@ -387,14 +484,14 @@ __global__ void __launch_bounds__(256) listed_kernel(const int64_t *__restrict__
 }
 
 // ---- products with dz: out[n][m] = sum_k A(k, m) B(n, k), A by columns ---------------------------------------------------------
-// split over k into gridDim.y ranges; partial sums to `part` [split][rows][ldp] (+= with `add`), or, unsplit, the result itself
+// split over k; partial sums to `part` [split][rows][ldp] (+= with `add`), or, unsplit, the result itself
 struct ProdArgs {
     Operand a, b;
     int64_t rows;                // n side
     int d;                       // m side
     int nseg;
-    int64_t ksteps;
-    int64_t tiles_m, tiles;
+    int64_t depth;               // K: the last step may reach beyond it, into zeros of dz
+    int64_t tiles_m, tiles, splits;
     float *part;
     int64_t ldp, part_stride;
     int add;
@@ -404,15 +501,13 @@ struct ProdArgs {
 };
 
 template <class TL, int DT>
-__global__ void __launch_bounds__(THREADS, 2) product_kernel(ProdArgs a)
+__device__ __forceinline__ void product(const ProdArgs &a, int64_t job, unsigned char *lds)
 {
-    __shared__ __attribute__((aligned(1024))) unsigned char lds[TL::LDS];
-    const int64_t t = xcd_tile(a.tiles);
-    if (t < 0) return;
+    const int64_t sp = job / a.tiles, t = job % a.tiles;
     const int64_t tm = t % a.tiles_m, tn = t / a.tiles_m;
     const int64_t m0 = tm * TL::BM, n0 = tn * TL::BN;
-    const int64_t steps = a.nseg * a.ksteps, splits = gridDim.y, sp = blockIdx.y;
-    const int64_t s0 = steps * sp / splits, s1 = steps * (sp + 1) / splits;
+    const int64_t ksteps = (a.depth + TL::KD - 1) / TL::KD, steps = a.nseg * ksteps;
+    const int64_t s0 = steps * sp / a.splits, s1 = steps * (sp + 1) / a.splits;
     Operand A = a.a, B = a.b;
     A.base += m0;
     A.lim = (int)((A.ld - m0) / 8 - 1);
@@ -423,12 +518,12 @@ __global__ void __launch_bounds__(THREADS, 2) product_kernel(ProdArgs a)
         B.base += n0 * B.ld;
         B.lim = TL::BN - 1;                     // (rows are padded to whole tiles)
     }
-    f32x4 acc[TL::MT][TL::NT];
+    typename TL::Acc acc;
 #pragma unroll
     for (int i = 0; i < TL::MT; ++i)
 #pragma unroll
         for (int j = 0; j < TL::NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    TL::run(acc, A, B, a.nseg, a.ksteps, s0, s1, lds);
+    TL::run(acc, A, B, a.nseg, ksteps, s0, s1, lds);
 
     const float f = a.part == nullptr ? a.top[0] * a.scale : 1.0f;
     const bool wide = (a.d & 7) == 0;
@@ -444,7 +539,8 @@ __global__ void __launch_bounds__(THREADS, 2) product_kernel(ProdArgs a)
                 float4 *p = (float4 *)(a.part + sp * a.part_stride + n * a.ldp + m);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    float4 v = {acc[4 * b + j][nt][0], acc[4 * b + j][nt][1], acc[4 * b + j][nt][2], acc[4 * b + j][nt][3]};
+                    const f32x4 r = TL::quad(acc, b, j, nt);
+                    float4 v = {r[0], r[1], r[2], r[3]};
                     if (a.add) {
                         const float4 o = p[j];
                         v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
@@ -459,7 +555,7 @@ __global__ void __launch_bounds__(THREADS, 2) product_kernel(ProdArgs a)
                     if (m + 8 * h >= a.d) continue;
                     float v[8];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] = acc[4 * b + 2 * h + (e >> 2)][nt][e & 3] * f;
+                    for (int e = 0; e < 8; ++e) v[e] = TL::quad(acc, b, 2 * h + (e >> 2), nt)[e & 3] * f;
                     if (DT == T_F32) {
                         float4 *o = (float4 *)((float *)a.out + n * a.d + m + 8 * h);
                         o[0] = float4{v[0], v[1], v[2], v[3]};
@@ -474,9 +570,27 @@ __global__ void __launch_bounds__(THREADS, 2) product_kernel(ProdArgs a)
             } else {
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
-                    if (m + e < a.d) store1<DT>(a.out, n * a.d + m + e, acc[4 * b + (e >> 2)][nt][e & 3] * f);
+                    if (m + e < a.d) store1<DT>(a.out, n * a.d + m + e, TL::quad(acc, b, e >> 2, nt)[e & 3] * f);
             }
         }
+    }
+}
+
+// dw of a piece (TW) and its share of dx (TX) in one launch: together they fill the chip with workgroups of about the same number
+// of steps, and dz is read by both while it is still in the last-level cache
+template <class TW, class TX, int DT>
+__global__ void __launch_bounds__(TW::THREADS, TW::OCCUPANCY) products_kernel(ProdArgs w, ProdArgs x)
+{
+    static_assert(TW::LDS == TX::LDS && TW::THREADS == TX::THREADS, "one workgroup shape");
+    __shared__ __attribute__((aligned(1024))) unsigned char lds[TW::LDS];
+    // each XCD: a contiguous eighth of either list
+    const int64_t xcd = blockIdx.x & 7, i = blockIdx.x >> 3;
+    const int64_t jobs_w = w.tiles * w.splits, jobs_x = x.tiles * x.splits, per_w = (jobs_w + 7) / 8, per_x = (jobs_x + 7) / 8;
+    if (i < per_w) {
+        if (xcd * per_w + i < jobs_w) product<TW, DT>(w, xcd * per_w + i, lds);
+    } else {
+        const int64_t j = i - per_w;
+        if (j < per_x && xcd * per_x + j < jobs_x) product<TX, DT>(x, xcd * per_x + j, lds);
     }
 }
 
@@ -511,12 +625,11 @@ __global__ void __launch_bounds__(256) join_kernel(const float *__restrict__ par
 int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
 
 struct Plan {
-    int64_t n, v, n_pad, vc;         // vc: classes of a piece (whole piece stride)
+    int64_t n, v, n_pad, vf, vc;     // vf, vc: classes of a piece, forward and backward (whole piece stride)
     int d, dp, parts, dtype;
     bool direct;                     // operands are read where they are
     bool small;                      // few rows: tiles of 32 rows
     int bm;                          // width of the d side of the products' tiles
-    int64_t k_dx, k_dw;              // K steps per segment
     int split_dx, split_dw;
 };
 
@@ -525,42 +638,39 @@ Plan make_plan(int64_t n, int64_t v, int d, int dtype)
     Plan p;
     p.n = n; p.v = v; p.d = d; p.dtype = dtype;
     p.parts = dtype == T_F32 ? 3 : 1;
-    p.dp = (int)up(d, 32);
-    p.direct = dtype != T_F32 && d % 32 == 0;
+    p.dp = (int)up(d, 64);
+    p.direct = dtype != T_F32 && d % 64 == 0;
     p.n_pad = up(n, 256);
     p.small = n <= 32;
-    int64_t most = DZ_BYTES / (p.n_pad * 2 * p.parts);
-    if (!p.direct) {
-        const int64_t m2 = WPACK_BYTES / ((int64_t)p.dp * 2 * p.parts);
-        most = most < m2 ? most : m2;
-    }
+    int64_t most = DZ_BYTES / (p.n_pad * 2 * p.parts), packed = WPACK_BYTES / ((int64_t)p.dp * 2 * p.parts) / 256 * 256;
+    if (packed < 256) packed = 256;
+    if (!p.direct && packed < most) most = packed;
     most = most / 256 * 256;
     if (most < 256) most = 256;
-    p.vc = up(v, 256) < most ? up(v, 256) : most;
+    // forward: nothing is kept of a piece but the packed codes; direct, one launch takes them all (bounded by the grid)
+    p.vf = p.direct ? 256ll * ((1ll << 22) / ((n + 31) / 32)) : packed;
+    if (p.vf < 256) p.vf = 256;
+    p.vf = p.vf < up(v, 256) ? p.vf : up(v, 256);
+    const int64_t pieces = (v + most - 1) / most;
+    p.vc = up((v + pieces - 1) / pieces, 256);
     p.bm = d > 128 ? 256 : (d > 64 ? 128 : 64);
-    const int bn = p.bm == 64 ? 256 : 128;
-    // enough workgroups for two per CU, but at least 8 K steps each
-    const int64_t want = 512;
-    auto splits = [&](int64_t tiles, int64_t steps) {
-        int64_t s = (want + tiles - 1) / tiles;
-        s = s < steps / 8 ? s : steps / 8;
+    // The products of a piece are cut over k into jobs of about the same number of steps (64 deep), so many that they
+    // fill the chip once (BM 256: one workgroup per CU, else two), none below 4 steps.
+    const int bn = p.bm == 128 ? 128 : 256;
+    const int64_t tm = (p.dp + p.bm - 1) / p.bm, seg = p.parts == 3 ? 6 : 1;
+    const int64_t tiles_w = tm * ((p.vc + bn - 1) / bn), tiles_x = tm * ((n + bn - 1) / bn);
+    const int64_t steps_w = seg * (up(n, 64) / 64), steps_x = seg * (p.vc / 64);
+    int64_t job = (tiles_w * steps_w + tiles_x * steps_x) / (p.bm == 256 ? 256 : 512);
+    job = job < 4 ? 4 : job;
+    auto splits = [&](int64_t steps) {
+        const int64_t s = (steps + job / 2) / job;
         return (int)(s < 1 ? 1 : (s > 64 ? 64 : s));
     };
-    const int64_t tm = (p.dp + p.bm - 1) / p.bm;
-    const int seg = p.parts == 3 ? 6 : 1;
-    p.k_dx = p.vc / BK;
-    p.k_dw = up(n, BK) / BK;
-    p.split_dx = splits(tm * ((n + bn - 1) / bn), seg * p.k_dx);
-    p.split_dw = splits(tm * ((p.vc + bn - 1) / bn), seg * p.k_dw);
+    p.split_dx = splits(steps_x);
+    p.split_dw = splits(steps_w);
     return p;
 }
 
-// classes of one forward launch without packed codes: as many as a grid of 2^22 tiles holds
-int64_t fwd_piece(const Plan &p)
-{
-    const int64_t tiles = (1ll << 22) / ((p.n + 31) / 32);
-    return (tiles < 1 ? 1 : tiles) * 256;
-}
 
 struct Space {          // hands out 256-byte aligned ranges; with base == NULL only counts
     unsigned char *base;
@@ -580,7 +690,7 @@ FwdSpace fwd_space(const Plan &p, Space &s)
 {
     FwdSpace f;
     f.xp = p.direct ? nullptr : (unsigned short *)s.take(p.n_pad * p.dp * 2 * p.parts);
-    f.wp = p.direct ? nullptr : (unsigned short *)s.take(p.vc * p.dp * 2 * p.parts);
+    f.wp = p.direct ? nullptr : (unsigned short *)s.take(p.vf * p.dp * 2 * p.parts);
     f.stats = (float2 *)s.take(up(p.v, 256) / 256 * p.n * 8);
     f.loss = (float *)s.take(p.n * 4);
     return f;
@@ -614,49 +724,54 @@ template <class TL, bool DZ, int PARTS>
 void launch_head(HeadArgs a, hipStream_t st)
 {
     a.tiles_n = (a.n + TL::BN - 1) / TL::BN;
-    if (DZ) a.tiles_n = a.n_pad / TL::BN;       // (the padding rows of dz are written too: the products read them)
     a.tiles = (a.vc + TL::BM - 1) / TL::BM * a.tiles_n;
-    const unsigned g = (unsigned)(up(a.tiles, 8));
-    head_kernel<TL, DZ, PARTS><<<g, THREADS, 0, st>>>(a);
+    head_kernel<TL, DZ, PARTS><<<(unsigned)up(a.tiles, 8), TL::THREADS, 0, st>>>(a);
+}
+template <class TL, bool DZ, int PARTS>
+void launch_head_walk(HeadArgs a, hipStream_t st)
+{
+    a.tiles_n = (a.n + TL::BN - 1) / TL::BN;        // (dz: n_pad / BN, the padding rows are written too)
+    a.tiles = (a.vc + TL::BM - 1) / TL::BM * a.tiles_n;
+    const int64_t g = up(a.tiles, 8);
+    head_walk_kernel<TL, DZ, PARTS><<<(unsigned)(g < CUS ? g : CUS), TL::THREADS, 0, st>>>(a);
 }
 
+template <bool DZ, bool F16, int PARTS>
+void head_of(const Plan &p, const HeadArgs &a, hipStream_t st)
+{
+    if (!DZ && p.small) launch_head<Tile<256, 32, 4, 1, false, false, F16>, false, PARTS>(a, st);
+    else launch_head_walk<DuoTile<256, 256, 2, 4, false, false, F16>, DZ, PARTS>(a, st);
+}
 template <bool DZ>
 void head(const Plan &p, const HeadArgs &a, hipStream_t st)
 {
-    if (p.dtype == T_F16) {
-        if (!DZ && p.small) launch_head<Tile<256, 32, 4, false, false, true>, DZ, 1>(a, st);
-        else launch_head<Tile<256, 128, 2, false, false, true>, DZ, 1>(a, st);
-    } else if (p.dtype == T_BF16) {
-        if (!DZ && p.small) launch_head<Tile<256, 32, 4, false, false, false>, DZ, 1>(a, st);
-        else launch_head<Tile<256, 128, 2, false, false, false>, DZ, 1>(a, st);
-    } else {
-        if (!DZ && p.small) launch_head<Tile<256, 32, 4, false, false, false>, DZ, 3>(a, st);
-        else launch_head<Tile<256, 128, 2, false, false, false>, DZ, 3>(a, st);
-    }
+    if (p.dtype == T_F16) head_of<DZ, true, 1>(p, a, st);
+    else if (p.dtype == T_BF16) head_of<DZ, false, 1>(p, a, st);
+    else head_of<DZ, false, 3>(p, a, st);
 }
 
-template <class TL>
-void launch_product(const Plan &p, ProdArgs a, int splits, hipStream_t st)
+template <class TW, class TX>
+void launch_products(const Plan &p, ProdArgs w, ProdArgs x, hipStream_t st)
 {
-    a.tiles_m = (p.dp + TL::BM - 1) / TL::BM;
-    a.tiles = a.tiles_m * ((a.rows + TL::BN - 1) / TL::BN);
-    const dim3 g((unsigned)up(a.tiles, 8), (unsigned)splits);
-    if (p.dtype == T_F32) product_kernel<TL, T_F32><<<g, THREADS, 0, st>>>(a);
-    else if (TL::F16) product_kernel<TL, T_F16><<<g, THREADS, 0, st>>>(a);
-    else product_kernel<TL, T_BF16><<<g, THREADS, 0, st>>>(a);
+    w.tiles_m = x.tiles_m = (p.dp + TW::BM - 1) / TW::BM;
+    w.tiles = w.rows > 0 ? w.tiles_m * ((w.rows + TW::BN - 1) / TW::BN) : 0;
+    x.tiles = x.rows > 0 ? x.tiles_m * ((x.rows + TX::BN - 1) / TX::BN) : 0;
+    const unsigned g = (unsigned)(8 * ((w.tiles * w.splits + 7) / 8 + (x.tiles * x.splits + 7) / 8));
+    if (p.dtype == T_F32) products_kernel<TW, TX, T_F32><<<g, TW::THREADS, 0, st>>>(w, x);
+    else if (TW::F16) products_kernel<TW, TX, T_F16><<<g, TW::THREADS, 0, st>>>(w, x);
+    else products_kernel<TW, TX, T_BF16><<<g, TW::THREADS, 0, st>>>(w, x);
 }
-template <bool BCOLS, bool F16>
-void product_w(const Plan &p, const ProdArgs &a, int splits, hipStream_t st)
+template <bool F16>
+void products_of(const Plan &p, const ProdArgs &w, const ProdArgs &x, hipStream_t st)
 {
-    if (p.bm == 64) launch_product<Tile<64, 256, 1, true, BCOLS, F16>>(p, a, splits, st);
-    else if (p.bm == 128) launch_product<Tile<128, 128, 2, true, BCOLS, F16>>(p, a, splits, st);
-    else launch_product<Tile<256, 128, 2, true, BCOLS, F16>>(p, a, splits, st);
+    if (p.bm == 64) launch_products<Tile<64, 256, 1, 4, true, true, F16>, Tile<64, 256, 1, 4, true, false, F16>>(p, w, x, st);
+    else if (p.bm == 128) launch_products<Tile<128, 128, 2, 2, true, true, F16>, Tile<128, 128, 2, 2, true, false, F16>>(p, w, x, st);
+    else launch_products<DuoTile<256, 256, 2, 4, true, true, F16>, DuoTile<256, 256, 2, 4, true, false, F16>>(p, w, x, st);
 }
-template <bool BCOLS>
-void product(const Plan &p, const ProdArgs &a, int splits, hipStream_t st)
+void products(const Plan &p, const ProdArgs &w, const ProdArgs &x, hipStream_t st)
 {
-    if (p.dtype == T_F16) product_w<BCOLS, true>(p, a, splits, st);
-    else product_w<BCOLS, false>(p, a, splits, st);
+    if (p.dtype == T_F16) products_of<true>(p, w, x, st);
+    else products_of<false>(p, w, x, st);
 }
 
 void join(const Plan &p, const float *part, int64_t stride, int splits, int64_t rows, const float *weight, const float *top,
@@ -716,18 +831,17 @@ int rsdf_class_head_fwd(const void *x, const void *w, int64_t n, int64_t v, int 
     const FwdSpace f = fwd_space(p, s);
     RSDF_CHECK_ARG(s.at <= workspace_bytes, "class_head_fwd: workspace too small");
     hipStream_t st = (hipStream_t)stream;
-    const int64_t xplane = p.n_pad * p.dp, wplane = p.vc * p.dp;
+    const int64_t xplane = p.n_pad * p.dp, wplane = p.vf * p.dp;
     if (!p.direct) pack(dtype, x, n, d, p.n_pad, p.dp, nullptr, f.xp, st);
-    const int64_t piece = p.direct ? fwd_piece(p) : p.vc;       // (nothing is kept of a piece but the packed codes)
-    for (int64_t v0 = 0; v0 < v; v0 += piece) {
-        const int64_t here = v - v0 < piece ? v - v0 : piece;
+    for (int64_t v0 = 0; v0 < v; v0 += p.vf) {
+        const int64_t here = v - v0 < p.vf ? v - v0 : p.vf;
         HeadArgs a = {};
-        if (!p.direct) pack(dtype, row_ptr(w, v0, d, dtype), here, d, p.vc, p.dp, nullptr, f.wp, st);
+        if (!p.direct) pack(dtype, row_ptr(w, v0, d, dtype), here, d, p.vf, p.dp, nullptr, f.wp, st);
         a.x = p.direct ? rows_of(x, 0, d) : rows_of(f.xp, xplane, p.dp);
         a.w = p.direct ? rows_of(row_ptr(w, v0, d, dtype), 0, d) : rows_of(f.wp, wplane, p.dp);
         a.n = n; a.vc = here;
         a.nseg = p.parts == 3 ? 6 : 1;
-        a.ksteps = p.dp / BK;
+        a.depth = p.dp;
         a.c = LOG2E / temperature;
         a.stats = f.stats;
         a.tile0 = v0 / 256;
@@ -772,7 +886,7 @@ int rsdf_class_head_bwd(const void *x, const void *w, int64_t n, int64_t v, int 
         a.w = p.direct ? rows_of(row_ptr(w, v0, d, dtype), 0, d) : rows_of(b.wp, wplane, p.dp);
         a.n = n; a.n_pad = p.n_pad; a.vc = here; a.ldz = p.vc;
         a.nseg = nseg;
-        a.ksteps = p.dp / BK;
+        a.depth = p.dp;
         a.c = LOG2E / temperature;
         a.lse = lse;
         a.weight = b.weight; a.top = b.top;
@@ -786,31 +900,32 @@ int rsdf_class_head_bwd(const void *x, const void *w, int64_t n, int64_t v, int 
             else if (dtype == T_BF16) listed_kernel<false, 1><<<g, 256, 0, st>>>(ids, q, listed_z, lse, b.weight, b.top, n, k, a.c, v0, p.vc, p.n_pad, b.dz);
             else listed_kernel<true, 1><<<g, 256, 0, st>>>(ids, q, listed_z, lse, b.weight, b.top, n, k, a.c, v0, p.vc, p.n_pad, b.dz);
         }
+        ProdArgs px = {}, pw = {};
+        px.splits = pw.splits = 1;
         if (dx != nullptr) {
-            ProdArgs r = {};
-            r.a = a.w;
-            r.a.k_rows = p.direct ? here : p.vc;
-            r.b = rows_of(b.dz, zplane, p.vc);
-            r.rows = n; r.d = d; r.nseg = nseg;
-            r.ksteps = up(here, BK) / BK;
-            r.part = b.dxp; r.ldp = p.dp; r.part_stride = n * p.dp; r.add = v0 > 0;
-            product<false>(p, r, p.split_dx, st);
+            px.a = a.w;
+            px.a.k_rows = (int)(p.direct ? here : p.vc);
+            px.b = rows_of(b.dz, zplane, p.vc);
+            px.rows = n; px.d = d; px.nseg = nseg;
+            px.depth = here;
+            px.splits = p.split_dx;
+            px.part = b.dxp; px.ldp = p.dp; px.part_stride = n * p.dp; px.add = v0 > 0;
         }
         if (dw != nullptr) {
-            ProdArgs r = {};
-            r.a = rows_of(b.xs, xplane, p.dp);
-            r.a.k_rows = p.n_pad;
-            r.b = rows_of(b.dz, zplane, p.vc);
-            r.b.k_rows = p.n_pad;
-            r.rows = here; r.d = d; r.nseg = nseg;
-            r.ksteps = p.k_dw;
-            r.part = b.dwp; r.ldp = p.dp; r.part_stride = p.vc * p.dp;
-            r.out = (unsigned char *)dw + v0 * d * (dtype == T_F32 ? 4 : 2);
-            r.top = b.top;
-            r.scale = scale;
-            product<true>(p, r, p.split_dw, st);
-            if (b.dwp != nullptr) join(p, b.dwp, r.part_stride, p.split_dw, here, nullptr, b.top, scale, r.out, st);
+            pw.a = rows_of(b.xs, xplane, p.dp);
+            pw.a.k_rows = (int)p.n_pad;
+            pw.b = rows_of(b.dz, zplane, p.vc);
+            pw.b.k_rows = (int)p.n_pad;
+            pw.rows = here; pw.d = d; pw.nseg = nseg;
+            pw.depth = n;
+            pw.splits = p.split_dw;
+            pw.part = b.dwp; pw.ldp = p.dp; pw.part_stride = p.vc * p.dp;
+            pw.out = (unsigned char *)dw + v0 * d * (dtype == T_F32 ? 4 : 2);
+            pw.top = b.top;
+            pw.scale = scale;
         }
+        products(p, pw, px, st);
+        if (b.dwp != nullptr) join(p, b.dwp, pw.part_stride, p.split_dw, here, nullptr, b.top, scale, pw.out, st);
     }
     if (dx != nullptr) join(p, b.dxp, n * p.dp, p.split_dx, n, b.weight, b.top, scale, dx, st);
     RSDF_RETURN_LAUNCH();
