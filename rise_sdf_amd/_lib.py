@@ -328,6 +328,16 @@ def stream_ptr():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
+def launch(device_index, fn, what, *args):
+    """``fn(*args, stream)`` on the current stream of device ``device_index`` (which need not be the current device), checked.
+    Pointers are plain integers here: the caller's tensors stay alive in its own variables until the call has returned."""
+    if torch._C._cuda_getDevice() == device_index:
+        check(fn(*args, torch._C._cuda_getCurrentRawStream(device_index)), what)
+    else:
+        with torch.cuda.device(device_index):
+            check(fn(*args, torch._C._cuda_getCurrentRawStream(device_index)), what)
+
+
 # ---- transient workspaces -----------------------------------------------------------------------------------------------
 # The fused SDF field's backward needs three large buffers that live only inside one backward call: the gradient planes
 # (896 B per sample), the hash backward's record queues (~1.9 KB per sample) and d(h2) (4 H B per sample) -- 48 of the ~88
@@ -468,14 +478,18 @@ def status(device) -> "torch.Tensor":
     return t
 
 
-def bad_ids_ptr(device):
-    """Where kernels count ids outside their table (status word ST_BAD_IDS).  None while a graph is being captured on a device
-    that has no status words yet: they would live in the graph's private pool."""
-    dev = torch.device(device)
-    idx = dev.index if dev.index is not None else torch.cuda.current_device()
-    if idx not in _STATUS and torch.cuda.is_current_stream_capturing():
-        return None
-    return ptr(status(dev)[ST_BAD_IDS:])
+_BAD_IDS_PTR = {}
+
+
+def bad_ids_ptr(idx):
+    """Address where kernels on device ``idx`` count ids outside their table (status word ST_BAD_IDS).  None while a graph is being
+    captured on a device that has no status words yet: they would live in the graph's private pool."""
+    p = _BAD_IDS_PTR.get(idx)
+    if p is None:
+        if idx not in _STATUS and torch.cuda.is_current_stream_capturing():
+            return None
+        p = _BAD_IDS_PTR[idx] = status(torch.device("cuda", idx)).data_ptr() + 4 * ST_BAD_IDS
+    return p
 
 
 def _status_delta(idx, vals):

@@ -32,6 +32,8 @@ constexpr int T_F32 = 0, T_BF16 = 1, T_F16 = 2;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float F16_DZ = 4096.0f;
 constexpr int64_t DZ_BYTES = 128ll << 20;      // of one piece of dz
+constexpr int MIN_JOB = 12;                     // steps of 64: 4 / 8 / 16 / 24 took 38.3 / 31.4 / 26.4 / 29.2 us of products and joining at
+                                                // 4096 x 1000 x 48 fp32, 44.8 / 41.1 / 38.7 / 45.1 at 1001 x 10007 x 200 fp16
 constexpr int CUS = 256;                        // MI355X
 constexpr int64_t WPACK_BYTES = 128ll << 20;   // of the packed class codes of one piece
 
@@ -81,23 +83,75 @@ __device__ __forceinline__ int64_t xcd_tile(int64_t total)
     return (b / 8 < per && i < total) ? i : -1;
 }
 
-// ---- operands: [rows][d] of any type -> 16-bit parts [P][rows_pad][dp], zero padded -----------------------------------------
-// weight (may be NULL): a row of weight 0 becomes zero whatever it holds
-template <int DT>
-__global__ void __launch_bounds__(256) pack_kernel(const void *__restrict__ src, int64_t rows, int d, int64_t rows_pad, int dp,
-                                                   const float *__restrict__ weight, unsigned short *__restrict__ dst)
+__device__ __forceinline__ float wave_max(float v)
 {
-    const int per = dp / 8;
-    const int64_t total = rows_pad * per;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t r = i / per;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+    return v;
+}
+
+// ---- before a pass, in one launch: operands as 16-bit parts, row weights -----------------------------------------------------
+// [rows][d] of any type -> [P][rows_pad][dp], zero padded.  lse (may be NULL): the rows are those of the gradient; one that takes
+// part in nothing, or has no weight, becomes zero whatever it holds.
+struct Pack { const void *src; int64_t rows, rows_pad; unsigned short *dst; };
+struct PrepArgs {
+    Pack p[2];
+    int64_t chunks[2];           // 8-element chunks of the two
+    int d, dp, wide;
+    // weight of a row in the gradient: T g_n (mean: / count), 0 where it takes part in nothing; top[0] = the largest |weight|
+    const float *lse, *g, *count;
+    int g_per_row;
+    float temperature;
+    int64_t n;
+    float *weight, *top;         // NULL: a forward pass
+};
+constexpr int PREP = 1024;
+
+template <int DT>
+__global__ void __launch_bounds__(PREP) prep_kernel(PrepArgs a)
+{
+    if (a.weight != nullptr && blockIdx.x == 0) {
+        __shared__ float sm[PREP / 64];
+        const float f = a.count != nullptr ? a.temperature / a.count[0] : a.temperature;
+        float m = 0.0f;
+        for (int64_t i = threadIdx.x; i < a.n; i += PREP) {
+            const float wr = a.lse[i] != __builtin_inff() ? a.g[a.g_per_row ? i : 0] * f : 0.0f;
+            a.weight[i] = wr;
+            m = fmaxf(m, fabsf(wr));
+        }
+        m = wave_max(m);
+        if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = m;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            for (int i = 0; i < PREP / 64; ++i) m = fmaxf(m, sm[i]);
+            a.top[0] = m > 0.0f ? m : 1.0f;
+        }
+        return;
+    }
+    const int64_t blocks = gridDim.x - (a.weight != nullptr), block = blockIdx.x - (a.weight != nullptr);
+    const int per = a.dp / 8;
+    for (int64_t j = block * PREP + threadIdx.x; j < a.chunks[0] + a.chunks[1]; j += blocks * PREP) {
+        const bool second = j >= a.chunks[0];
+        const Pack &p = a.p[second];
+        const int64_t i = second ? j - a.chunks[0] : j, r = i / per;
         const int c = (int)(i % per) * 8;
-        const bool live = r < rows && (weight == nullptr || weight[r] != 0.0f);
+        bool live = r < p.rows;
+        if (live && !second && a.lse != nullptr) live = a.lse[r] != __builtin_inff() && a.g[a.g_per_row ? r : 0] != 0.0f;
+        float x[8];
+        if (live && a.wide && c + 8 <= a.d) {        // (rows are whole 16-byte pieces)
+            const u32x4 *s = (const u32x4 *)((const unsigned char *)p.src + (r * a.d + c) * (DT == T_F32 ? 4 : 2));
+            u32x4 raw[2] = {s[0], s[0]};
+            if (DT == T_F32) raw[1] = s[1];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = load1<DT>(raw, e);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = live && c + e < a.d ? load1<DT>(p.src, r * a.d + c + e) : 0.0f;
+        }
         unsigned short o[3][8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            float v = 0.0f;
-            if (live && c + e < d) v = load1<DT>(src, r * d + c + e);
+            const float v = x[e];
             if (DT == T_F32) {
                 unsigned short h[3];
                 split3(v, h);
@@ -107,7 +161,7 @@ __global__ void __launch_bounds__(256) pack_kernel(const void *__restrict__ src,
             }
         }
 #pragma unroll
-        for (int p = 0; p < (DT == T_F32 ? 3 : 1); ++p) *(u32x4 *)(dst + (p * rows_pad + r) * dp + c) = *(const u32x4 *)o[p];
+        for (int k = 0; k < (DT == T_F32 ? 3 : 1); ++k) *(u32x4 *)(p.dst + (k * p.rows_pad + r) * a.dp + c) = *(const u32x4 *)o[k];
     }
 }
 
@@ -139,6 +193,7 @@ __device__ __forceinline__ void head_tile(const HeadArgs &a, int64_t t, Operand 
     n0 = t % a.tiles_n * TL::BN;
     W = a.w;
     X = a.x;
+    if (m0 >= a.vc || n0 >= a.n) return;        // (nothing to read: a tile of zeros)
     W.base += m0 * W.ld;
     W.lim = (int)(a.vc - 1 - m0 < TL::BM - 1 ? a.vc - 1 - m0 : TL::BM - 1);
     X.base += n0 * X.ld;
@@ -172,7 +227,7 @@ __device__ __forceinline__ void head_results(const HeadArgs &a, typename TL::Acc
                                              float2 *part /* [WM][BN], LDS */)
 {
     const bool whole = a.vc - m0 >= TL::BM;     // else the last classes of the tile are not there
-    const int left = whole ? TL::BM : (int)(a.vc - m0);
+    const int left = whole ? TL::BM : (int)(a.vc - m0);      // (0 or less: a tile of zeros)
     if (!DZ) {
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / TL::WN;
         if (!whole) {
@@ -283,7 +338,8 @@ __global__ void __launch_bounds__(TL::THREADS, TL::OCCUPANCY) head_kernel(HeadAr
     typename TL::Acc acc;
     clear<TL>(acc);
     const int64_t ksteps = a.depth / TL::KD;
-    TL::run(acc, W, X, a.nseg, ksteps, 0, a.nseg * ksteps, lds);
+    const bool there = m0 < a.vc && n0 < a.n;
+    TL::run(acc, W, X, a.nseg, ksteps, 0, there ? a.nseg * ksteps : 0, lds);
     RowState<TL> rows;
     if (DZ) rows.load(a, m0, n0);
     head_results<TL, DZ, PARTS>(a, acc, rows, m0, n0, (float2 *)lds);
@@ -339,79 +395,144 @@ struct RowArgs {
     int *status;                 // counts ids outside [0, v); may be NULL
 };
 
-__device__ __forceinline__ float wave_max(float v)
+// G dot products of row x with G rows of w by one wave: lane l gets number (l >> 3) & 7 of them.  The eight sums are folded
+// together, so that they cost 10 exchanges instead of 48.
+constexpr int G = 8;
+template <int DT, bool VEC>
+__device__ __forceinline__ float dots(const void *x, const void *w, int64_t xo, const int64_t (&wo)[G], int d)
 {
+    constexpr int E = VEC ? (DT == T_F32 ? 4 : 8) : 1;
+    const int lane = threadIdx.x & 63;
+    float s[G];
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-    return v;
+    for (int j = 0; j < G; ++j) s[j] = 0.0f;
+    for (int i = lane * E; i < d; i += 64 * E) {
+        float a[E];
+        if (VEC) {
+            const u32x4 r = *(const u32x4 *)((const unsigned char *)x + (xo + i) * (DT == T_F32 ? 4 : 2));
+#pragma unroll
+            for (int e = 0; e < E; ++e) a[e] = load1<DT>(&r, e);
+        } else {
+            a[0] = load1<DT>(x, xo + i);
+        }
+        u32x4 b[G];
+        if (VEC) {
+#pragma unroll
+            for (int j = 0; j < G; ++j) b[j] = *(const u32x4 *)((const unsigned char *)w + (wo[j] + i) * (DT == T_F32 ? 4 : 2));
+        }
+#pragma unroll
+        for (int j = 0; j < G; ++j)
+#pragma unroll
+            for (int e = 0; e < E; ++e) s[j] = fmaf(a[e], VEC ? load1<DT>(&b[j], e) : load1<DT>(w, wo[j] + i), s[j]);
+    }
+#pragma unroll
+    for (int o = 32, m = G / 2; m >= 1; o >>= 1, m >>= 1)
+#pragma unroll
+        for (int j = 0; j < m; ++j) {
+            const bool up = lane & o;
+            s[j] = (up ? s[j + m] : s[j]) + __shfl_xor(up ? s[j] : s[j + m], o, 64);
+        }
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) s[0] += __shfl_xor(s[0], o, 64);
+    return s[0];
 }
 
-template <int DT>
-__device__ __forceinline__ float dot_row(const void *x, const void *w, int64_t xo, int64_t wo, int d)
-{
-    float s = 0.0f;
-    for (int i = threadIdx.x & 63; i < d; i += 64) s = fmaf(load1<DT>(x, xo + i), load1<DT>(w, wo + i), s);
-    return wave_sum(s);
-}
-
-template <int DT>
+// LR rows per workgroup (4; 1 where a teacher's rows are few).  The tiles' statistics are read with rows running
+// fastest, then each wave takes whole rows (1 row: its waves share the listed classes).
+template <int DT, bool VEC, int LR>
 __global__ void __launch_bounds__(256) rows_kernel(RowArgs a)
 {
-    const int lane = threadIdx.x & 63;
-    const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (r >= a.n) return;
-    float2 st = {-__builtin_inff(), 0.0f};
-    for (int64_t t = lane; t < a.tiles; t += 64) st = join_stats(st, a.stats[t * a.n + r]);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) st = join_stats(st, float2{__shfl_xor(st.x, o, 64), __shfl_xor(st.y, o, 64)});
-    const float lse = st.x + __builtin_amdgcn_logf(st.y);     // v_log_f32: base 2
-    const float inv_t = 1.0f / a.temperature;
-    float loss = 0.0f;
-    bool alive = false, bad = false;
-    if (a.logits == nullptr) {
-        const int64_t id = a.ids[r];
-        bad = id != a.ignore && (id < 0 || id >= a.v);
-        alive = id != a.ignore && !bad;
-        if (alive) loss = lse * LN2 - dot_row<DT>(a.x, a.w, r * a.d, id * a.d, a.d);
-    } else {
-        const int64_t *ids = a.ids + r * a.k;
-        const float *lg = a.logits + r * a.k;
-        float *q = a.q + r * a.k, *zt = a.zt + r * a.k;
-        float tm = -__builtin_inff();
-        bool nan = false;
-        for (int k = lane; k < a.k; k += 64) {
-            if (ids[k] < 0) continue;               // (whatever its logit holds)
-            bad |= ids[k] >= a.v;
-            nan |= lg[k] != lg[k];
-            tm = fmaxf(tm, lg[k]);
+    __shared__ float2 st[256];
+    __shared__ float part[4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int64_t r0 = (int64_t)blockIdx.x * LR;
+    {
+        const int r = tid % LR;
+        float2 s = {-__builtin_inff(), 0.0f};
+        if (r0 + r < a.n)
+            for (int64_t t = tid / LR; t < a.tiles; t += 256 / LR) s = join_stats(s, a.stats[t * a.n + r0 + r]);
+        st[tid] = s;
+        __syncthreads();
+        for (int o = 128; o >= LR; o >>= 1) {
+            if (tid < o) st[tid] = join_stats(st[tid], st[tid + o]);
+            __syncthreads();
         }
-        tm = wave_max(tm);
-        bad = __any(bad);
-        alive = (tm > -__builtin_inff() || __any(nan)) && !bad;
-        float sum = 0.0f;
-        if (alive)
-            for (int k = lane; k < a.k; k += 64)
-                if (ids[k] >= 0) sum += expf((lg[k] - tm) * inv_t);     // (the difference first: logits at the type's ends)
-        sum = wave_sum(sum);
-        const float lse_e = lse * LN2, ls = logf(sum);
-        for (int k = 0; k < a.k; ++k) {
-            const int64_t id = ids[k];
-            float qk = 0.0f, z = 0.0f;
-            if (alive && id >= 0) {
-                const float lq = (lg[k] - tm) * inv_t - ls;
-                qk = expf(lq);
-                z = dot_row<DT>(a.x, a.w, r * a.d, id * a.d, a.d);
-                if (!(qk == 0.0f)) loss += qk * (lq - z * inv_t + lse_e);
-            }
-            if (lane == 0) { q[k] = qk; zt[k] = z; }
-        }
-        loss *= a.temperature * a.temperature;
     }
-    if (lane != 0) return;
-    if (bad) loss = __builtin_nanf("");
-    if (bad && a.status != nullptr) atomicAdd(a.status, 1);
-    a.loss[r] = loss;
-    a.lse[r] = alive ? lse : __builtin_inff();
+    const float inv_t = 1.0f / a.temperature;
+    for (int rr = LR == 1 ? 0 : wave; rr < LR; rr += 4) {
+        const int64_t r = r0 + rr;
+        if (r >= a.n) return;                       // (LR 1: r0 < n)
+        const float lse = st[rr].x + __builtin_amdgcn_logf(st[rr].y);     // v_log_f32: base 2
+        float loss = 0.0f;
+        bool alive = false, bad = false;
+        if (a.logits == nullptr) {
+            const int64_t id = a.ids[r];
+            bad = id != a.ignore && (id < 0 || id >= a.v);
+            alive = id != a.ignore && !bad;
+            if (alive) {
+                float s = 0.0f;
+                for (int i = lane; i < a.d; i += 64) s = fmaf(load1<DT>(a.x, r * a.d + i), load1<DT>(a.w, id * a.d + i), s);
+                loss = lse * LN2 - wave_sum(s);
+            }
+        } else {
+            const int64_t *ids = a.ids + r * a.k;
+            const float *lg = a.logits + r * a.k;
+            float *q = a.q + r * a.k, *zt = a.zt + r * a.k;
+            float tm = -__builtin_inff();
+            bool nan = false;
+            for (int k = lane; k < a.k; k += 64) {
+                if (ids[k] < 0) continue;           // (whatever its logit holds)
+                bad |= ids[k] >= a.v;
+                nan |= lg[k] != lg[k];
+                tm = fmaxf(tm, lg[k]);
+            }
+            tm = wave_max(tm);
+            bad = __any(bad);
+            alive = (tm > -__builtin_inff() || __any(nan)) && !bad;
+            float sum = 0.0f;
+            if (alive)
+                for (int k = lane; k < a.k; k += 64)
+                    if (ids[k] >= 0) sum += expf((lg[k] - tm) * inv_t);   // (the difference first: logits at the type's ends)
+            sum = wave_sum(sum);
+            const float lse_e = lse * LN2, ls = logf(sum);
+            for (int k0 = LR == 1 ? wave * G : 0; k0 < a.k; k0 += LR == 1 ? 4 * G : G) {
+                int64_t wo[G];
+#pragma unroll
+                for (int j = 0; j < G; ++j) {
+                    const int64_t id = k0 + j < a.k ? ids[k0 + j] : -1;
+                    wo[j] = (alive && id >= 0 ? id : 0) * a.d;            // (a class that is there; its product is not used)
+                }
+                float z = alive ? dots<DT, VEC>(a.x, a.w, r * a.d, wo, a.d) : 0.0f;
+                const int k = k0 + ((lane >> 3) & 7);
+                if (k < a.k && (lane & 7) == 0) {
+                    float qk = 0.0f;
+                    if (alive && ids[k] >= 0) {
+                        const float lq = (lg[k] - tm) * inv_t - ls;
+                        qk = expf(lq);
+                        if (!(qk == 0.0f)) loss += qk * (lq - z * inv_t + lse_e);
+                    } else {
+                        z = 0.0f;
+                    }
+                    q[k] = qk;
+                    zt[k] = z;
+                }
+            }
+            loss = wave_sum(loss);
+            if (LR == 1) {
+                if (lane == 0) part[wave] = loss;
+                __syncthreads();
+                loss = (part[0] + part[1]) + (part[2] + part[3]);
+                if (wave != 0) return;
+            }
+            loss *= a.temperature * a.temperature;
+        }
+        if (lane == 0) {
+            if (bad) loss = __builtin_nanf("");
+            if (bad && a.status != nullptr) atomicAdd(a.status, 1);
+            a.loss[r] = loss;
+            a.lse[r] = alive ? lse : __builtin_inff();
+        }
+    }
 }
 
 // sum of the rows' losses (and their number) in a fixed order: one block
@@ -438,49 +559,41 @@ __global__ void __launch_bounds__(1024) sum_kernel(const float *__restrict__ los
     }
 }
 
-// weight of a row in the gradient: T g_n (mean: / count), 0 where it takes part in nothing; top[0] = the largest |weight|
-__global__ void __launch_bounds__(1024) weights_kernel(const float *__restrict__ lse, const float *__restrict__ g, int g_per_row,
-                                                       const float *__restrict__ count, float temperature, int64_t n,
-                                                       float *__restrict__ weight, float *__restrict__ top)
-{
-    __shared__ float sm[16];
-    const float f = count != nullptr ? temperature / count[0] : temperature;
-    float m = 0.0f;
-    for (int64_t i = threadIdx.x; i < n; i += 1024) {
-        const float wr = lse[i] != __builtin_inff() ? g[g_per_row ? i : 0] * f : 0.0f;
-        weight[i] = wr;
-        m = fmaxf(m, fabsf(wr));
-    }
-    m = wave_max(m);
-    if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = m;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int i = 0; i < 16; ++i) m = fmaxf(m, sm[i]);
-        top[0] = m > 0.0f ? m : 1.0f;
-    }
-}
-
-// the listed classes' entries of dz: p - (sum of the q of that class in this row); a class listed twice is written twice alike
+// The listed classes' entries of dz: p - (sum of the q of that class in this row); a class listed twice is written twice alike.
+// One wave per row, its entries 64 at a time in the lanes.
 template <bool F16, int PARTS>
 __global__ void __launch_bounds__(256) listed_kernel(const int64_t *__restrict__ ids, const float *__restrict__ q,
                                                      const float *__restrict__ zt, const float *__restrict__ lse,
                                                      const float *__restrict__ weight, const float *__restrict__ top, int64_t n, int k,
                                                      float c, int64_t v0, int64_t vc, int64_t n_pad, unsigned short *__restrict__ dz)
 {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= n * k) return;
-    const int64_t r = i / k, id = ids[i];
+    const int lane = threadIdx.x & 63;
+    const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (r >= n) return;
     const float l = lse[r];
-    if (id < v0 || id >= v0 + vc || l == __builtin_inff()) return;
-    float s = 0.0f;
-    for (int j = 0; j < k; ++j) s += ids[r * k + j] == id ? q[r * k + j] : 0.0f;
-    if (s == 0.0f) return;
-    const float p = (__builtin_amdgcn_exp2f(zt[i] * c - l) - s) * (weight[r] / top[0] * (F16 ? F16_DZ : 1.0f));
-    unsigned short h[3];
-    if (PARTS == 3) split3(p, h);
-    else h[0] = to16<F16>(p);
+    if (l == __builtin_inff()) return;
+    const float f = weight[r] / top[0] * (F16 ? F16_DZ : 1.0f);
+    for (int k0 = 0; k0 < k; k0 += 64) {
+        const int i = k0 + lane;
+        const int64_t id = i < k ? ids[r * k + i] : -1;
+        float s = 0.0f;
+        for (int j0 = 0; j0 < k; j0 += 64) {
+            const int64_t jd = j0 == k0 ? id : (j0 + lane < k ? ids[r * k + j0 + lane] : -1);
+            const float jq = j0 + lane < k ? q[r * k + j0 + lane] : 0.0f;
+            const int here = k - j0 < 64 ? k - j0 : 64;
+            for (int j = 0; j < here; ++j) {        // (ids of this head fit 32 bits; absent ones match nothing that is written)
+                const float t = __shfl(jq, j, 64);
+                s += __shfl((int)jd, j, 64) == (int)id ? t : 0.0f;
+            }
+        }
+        if (id < v0 || id >= v0 + vc || s == 0.0f) continue;
+        const float p = f != 0.0f ? (__builtin_amdgcn_exp2f(zt[r * k + i] * c - l) - s) * f : 0.0f;
+        unsigned short h[3];
+        if (PARTS == 3) split3(p, h);
+        else h[0] = to16<F16>(p);
 #pragma unroll
-    for (int part = 0; part < PARTS; ++part) dz[(part * n_pad + r) * vc + id - v0] = h[part];
+        for (int part = 0; part < PARTS; ++part) dz[(part * n_pad + r) * vc + id - v0] = h[part];
+    }
 }
 
 // ---- products with dz: out[n][m] = sum_k A(k, m) B(n, k), A by columns ---------------------------------------------------------
@@ -594,30 +707,48 @@ __global__ void __launch_bounds__(TW::THREADS, TW::OCCUPANCY) products_kernel(Pr
     }
 }
 
-// out[r][c] = (sum over the splits) * top * scale; rows of weight 0 (weight may be NULL: none) are zero
+// out[r][c] = (sum over the splits) * top * scale, for up to two results; rows of weight 0 (weight may be NULL: none) are zero
+struct Join {
+    const float *part;
+    int64_t part_stride, rows;
+    int splits;
+    const float *weight;
+    void *out;
+};
 template <int DT>
-__global__ void __launch_bounds__(256) join_kernel(const float *__restrict__ part, int64_t part_stride, int splits, int64_t rows, int d,
-                                                   int64_t ldp, const float *__restrict__ weight, const float *__restrict__ top,
-                                                   float scale, void *__restrict__ out)
+__global__ void __launch_bounds__(256) join_kernel(Join ja, Join jb, int d, int64_t ldp, const float *__restrict__ top, float scale)
 {
     const int per = (int)(ldp / 4);
-    const int64_t total = rows * per;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t r = i / per;
+    const int64_t first = ja.rows * per, total = first + jb.rows * per;
+    const float g = top[0] * scale;
+    for (int64_t j = (int64_t)blockIdx.x * 256 + threadIdx.x; j < total; j += (int64_t)gridDim.x * 256) {
+        const bool second = j >= first;
+        const Join &a = second ? jb : ja;
+        const int64_t i = second ? j - first : j, r = i / per;
         const int c = (int)(i % per) * 4;
         if (c >= d) continue;
         float4 s = {0.f, 0.f, 0.f, 0.f};
-        if (weight == nullptr || weight[r] != 0.0f) {
-            for (int k = 0; k < splits; ++k) {
-                const float4 p = *(const float4 *)(part + k * part_stride + r * ldp + c);
-                s.x += p.x; s.y += p.y; s.z += p.z; s.w += p.w;
+        if (a.weight == nullptr || a.weight[r] != 0.0f) {
+            const float *p = a.part + r * ldp + c;
+#pragma unroll 4
+            for (int k = 0; k < a.splits; ++k) {
+                const float4 v = *(const float4 *)(p + k * a.part_stride);
+                s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
             }
-            const float g = top[0] * scale;
-            s.x *= g; s.y *= g; s.z *= g; s.w *= g;
         }
-        const float v[4] = {s.x, s.y, s.z, s.w};
+        const float v[4] = {s.x * g, s.y * g, s.z * g, s.w * g};
+        if ((d & 3) == 0) {
+            if (DT == T_F32) {
+                *(float4 *)((float *)a.out + r * d + c) = float4{v[0], v[1], v[2], v[3]};
+            } else {
+                unsigned short u[4];
+                for (int e = 0; e < 4; ++e) u[e] = to16<DT == T_F16>(v[e]);
+                *(uint2 *)((unsigned short *)a.out + r * d + c) = *(const uint2 *)u;
+            }
+            continue;
+        }
         for (int e = 0; e < 4; ++e)
-            if (c + e < d) store1<DT>(out, r * d + c + e, v[e]);
+            if (c + e < d) store1<DT>(a.out, r * d + c + e, v[e]);
     }
 }
 
@@ -625,6 +756,8 @@ __global__ void __launch_bounds__(256) join_kernel(const float *__restrict__ par
 int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
 
 struct Plan {
+    int sbm;                         // classes of a forward tile
+    bool quarter;                    // few tiles: 128 x 128 ones
     int64_t n, v, n_pad, vf, vc;     // vf, vc: classes of a piece, forward and backward (whole piece stride)
     int d, dp, parts, dtype;
     bool direct;                     // operands are read where they are
@@ -642,6 +775,8 @@ Plan make_plan(int64_t n, int64_t v, int d, int dtype)
     p.direct = dtype != T_F32 && d % 64 == 0;
     p.n_pad = up(n, 256);
     p.small = n <= 32;
+    p.quarter = up(n, 256) / 256 * (up(v, 256) / 256) <= CUS;      // (4096 x 1000 x 48 fp32: 26 instead of 44 us of tiles)
+    p.sbm = p.quarter && !p.small ? 128 : 256;
     int64_t most = DZ_BYTES / (p.n_pad * 2 * p.parts), packed = WPACK_BYTES / ((int64_t)p.dp * 2 * p.parts) / 256 * 256;
     if (packed < 256) packed = 256;
     if (!p.direct && packed < most) most = packed;
@@ -655,19 +790,23 @@ Plan make_plan(int64_t n, int64_t v, int d, int dtype)
     p.vc = up((v + pieces - 1) / pieces, 256);
     p.bm = d > 128 ? 256 : (d > 64 ? 128 : 64);
     // The products of a piece are cut over k into jobs of about the same number of steps (64 deep), so many that they
-    // fill the chip once (BM 256: one workgroup per CU, else two), none below 4 steps.
+    // fill the chip once (BM 256: one workgroup per CU, else two), none below MIN_JOB steps.
     const int bn = p.bm == 128 ? 128 : 256;
     const int64_t tm = (p.dp + p.bm - 1) / p.bm, seg = p.parts == 3 ? 6 : 1;
     const int64_t tiles_w = tm * ((p.vc + bn - 1) / bn), tiles_x = tm * ((n + bn - 1) / bn);
     const int64_t steps_w = seg * (up(n, 64) / 64), steps_x = seg * (p.vc / 64);
-    int64_t job = (tiles_w * steps_w + tiles_x * steps_x) / (p.bm == 256 ? 256 : 512);
-    job = job < 4 ? 4 : job;
+    const int64_t slots = p.bm == 256 ? CUS : 2 * CUS;
+    int64_t job = (tiles_w * steps_w + tiles_x * steps_x + slots - 1) / slots;
+    job = job < MIN_JOB ? MIN_JOB : job;
     auto splits = [&](int64_t steps) {
-        const int64_t s = (steps + job / 2) / job;
+        const int64_t s = (steps + job - 1) / job;
         return (int)(s < 1 ? 1 : (s > 64 ? 64 : s));
     };
-    p.split_dx = splits(steps_x);
-    p.split_dw = splits(steps_w);
+    for (;; ++job) {
+        p.split_dx = splits(steps_x);
+        p.split_dw = splits(steps_w);
+        if (tiles_w * p.split_dw + tiles_x * p.split_dx <= slots || (p.split_dw == 1 && p.split_dx == 1)) break;
+    }
     return p;
 }
 
@@ -684,14 +823,14 @@ struct Space {          // hands out 256-byte aligned ranges; with base == NULL 
 };
 
 struct FwdSpace { unsigned short *xp, *wp; float2 *stats; float *loss; };
-struct BwdSpace { unsigned short *xs, *xp, *wp, *dz; float *dxp, *dwp, *weight, *top; };
+struct BwdSpace { unsigned short *xs, *wp, *dz; float *dxp, *dwp, *weight, *top; };
 
 FwdSpace fwd_space(const Plan &p, Space &s)
 {
     FwdSpace f;
     f.xp = p.direct ? nullptr : (unsigned short *)s.take(p.n_pad * p.dp * 2 * p.parts);
     f.wp = p.direct ? nullptr : (unsigned short *)s.take(p.vf * p.dp * 2 * p.parts);
-    f.stats = (float2 *)s.take(up(p.v, 256) / 256 * p.n * 8);
+    f.stats = (float2 *)s.take((p.v + p.sbm - 1) / p.sbm * p.n * 8);
     f.loss = (float *)s.take(p.n * 4);
     return f;
 }
@@ -700,31 +839,35 @@ BwdSpace bwd_space(const Plan &p, Space &s, bool dx, bool dw)
     BwdSpace b;
     b.weight = (float *)s.take(p.n * 4);
     b.top = (float *)s.take(4);
-    b.xp = p.direct ? nullptr : (unsigned short *)s.take(p.n_pad * p.dp * 2 * p.parts);
     b.wp = p.direct ? nullptr : (unsigned short *)s.take(p.vc * p.dp * 2 * p.parts);
-    b.xs = dw ? (unsigned short *)s.take(p.n_pad * p.dp * 2 * p.parts) : nullptr;
+    b.xs = dw || !p.direct ? (unsigned short *)s.take(p.n_pad * p.dp * 2 * p.parts) : nullptr;
     b.dz = (unsigned short *)s.take(p.n_pad * p.vc * 2 * p.parts);
     b.dxp = dx ? (float *)s.take(p.split_dx * p.n * (int64_t)p.dp * 4) : nullptr;
     b.dwp = dw && p.split_dw > 1 ? (float *)s.take(p.split_dw * p.vc * (int64_t)p.dp * 4) : nullptr;
     return b;
 }
 
-unsigned grid1(int64_t items) { const int64_t b = (items + 255) / 256; return (unsigned)(b < 1 ? 1 : (b > 8192 ? 8192 : b)); }
-
-void pack(int dtype, const void *src, int64_t rows, int d, int64_t rows_pad, int dp, const float *weight, unsigned short *dst,
-          hipStream_t st)
+void prep(int dtype, const PrepArgs &a, hipStream_t st)
 {
-    const unsigned g = grid1(rows_pad * (dp / 8));
-    if (dtype == T_F32) pack_kernel<T_F32><<<g, 256, 0, st>>>(src, rows, d, rows_pad, dp, weight, dst);
-    else if (dtype == T_BF16) pack_kernel<T_BF16><<<g, 256, 0, st>>>(src, rows, d, rows_pad, dp, weight, dst);
-    else pack_kernel<T_F16><<<g, 256, 0, st>>>(src, rows, d, rows_pad, dp, weight, dst);
+    int64_t g = (a.chunks[0] + a.chunks[1] + PREP - 1) / PREP;
+    g = (g > 4 * CUS ? 4 * CUS : g) + (a.weight != nullptr);
+    if (g == 0) return;
+    if (dtype == T_F32) prep_kernel<T_F32><<<(unsigned)g, PREP, 0, st>>>(a);
+    else if (dtype == T_BF16) prep_kernel<T_BF16><<<(unsigned)g, PREP, 0, st>>>(a);
+    else prep_kernel<T_F16><<<(unsigned)g, PREP, 0, st>>>(a);
+}
+void add_pack(PrepArgs &a, int i, const void *src, int64_t rows, int64_t rows_pad, unsigned short *dst)
+{
+    a.p[i] = Pack{src, rows, rows_pad, dst};
+    a.chunks[i] = rows_pad * (a.dp / 8);
 }
 
 template <class TL, bool DZ, int PARTS>
 void launch_head(HeadArgs a, hipStream_t st)
 {
-    a.tiles_n = (a.n + TL::BN - 1) / TL::BN;
-    a.tiles = (a.vc + TL::BM - 1) / TL::BM * a.tiles_n;
+    // dz: the products read whole blocks of 256 rows and classes, so the tiles beyond the last ones write zeros
+    a.tiles_n = ((DZ ? a.n_pad : a.n) + TL::BN - 1) / TL::BN;
+    a.tiles = ((DZ ? up(a.vc, 256) : a.vc) + TL::BM - 1) / TL::BM * a.tiles_n;
     head_kernel<TL, DZ, PARTS><<<(unsigned)up(a.tiles, 8), TL::THREADS, 0, st>>>(a);
 }
 template <class TL, bool DZ, int PARTS>
@@ -740,6 +883,7 @@ template <bool DZ, bool F16, int PARTS>
 void head_of(const Plan &p, const HeadArgs &a, hipStream_t st)
 {
     if (!DZ && p.small) launch_head<Tile<256, 32, 4, 1, false, false, F16>, false, PARTS>(a, st);
+    else if (p.quarter) launch_head<Tile<128, 128, 2, 2, false, false, F16>, DZ, PARTS>(a, st);
     else launch_head_walk<DuoTile<256, 256, 2, 4, false, false, F16>, DZ, PARTS>(a, st);
 }
 template <bool DZ>
@@ -774,13 +918,29 @@ void products(const Plan &p, const ProdArgs &w, const ProdArgs &x, hipStream_t s
     else products_of<false>(p, w, x, st);
 }
 
-void join(const Plan &p, const float *part, int64_t stride, int splits, int64_t rows, const float *weight, const float *top,
-          float scale, void *out, hipStream_t st)
+void join(const Plan &p, const Join &a, const Join &b, const float *top, float scale, hipStream_t st)
 {
-    const unsigned g = grid1(rows * (p.dp / 4));
-    if (p.dtype == T_F32) join_kernel<T_F32><<<g, 256, 0, st>>>(part, stride, splits, rows, p.d, p.dp, weight, top, scale, out);
-    else if (p.dtype == T_BF16) join_kernel<T_BF16><<<g, 256, 0, st>>>(part, stride, splits, rows, p.d, p.dp, weight, top, scale, out);
-    else join_kernel<T_F16><<<g, 256, 0, st>>>(part, stride, splits, rows, p.d, p.dp, weight, top, scale, out);
+    const int64_t items = (a.rows + b.rows) * (p.dp / 4);
+    if (items == 0) return;
+    const int64_t blocks = (items + 255) / 256;
+    const unsigned g = (unsigned)(blocks > 8192 ? 8192 : blocks);
+    if (p.dtype == T_F32) join_kernel<T_F32><<<g, 256, 0, st>>>(a, b, p.d, p.dp, top, scale);
+    else if (p.dtype == T_BF16) join_kernel<T_BF16><<<g, 256, 0, st>>>(a, b, p.d, p.dp, top, scale);
+    else join_kernel<T_F16><<<g, 256, 0, st>>>(a, b, p.d, p.dp, top, scale);
+}
+
+template <int DT, bool VEC>
+void launch_rows(const RowArgs &r, hipStream_t st)
+{
+    if (r.logits == nullptr || r.n >= 2 * CUS) rows_kernel<DT, VEC, 4><<<(unsigned)((r.n + 3) / 4), 256, 0, st>>>(r);
+    else rows_kernel<DT, VEC, 1><<<(unsigned)r.n, 256, 0, st>>>(r);
+}
+void rows_pass(int dtype, const RowArgs &r, hipStream_t st)
+{
+    // 16-byte loads of rows: x and w are aligned, so a row is where its length is
+    if (dtype == T_F32) r.d % 4 == 0 ? launch_rows<T_F32, true>(r, st) : launch_rows<T_F32, false>(r, st);
+    else if (dtype == T_BF16) r.d % 8 == 0 ? launch_rows<T_BF16, true>(r, st) : launch_rows<T_BF16, false>(r, st);
+    else r.d % 8 == 0 ? launch_rows<T_F16, true>(r, st) : launch_rows<T_F16, false>(r, st);
 }
 
 const char *bad_head(int64_t n, int64_t v, int d, int dtype, int k, const void *x, const void *w)
@@ -832,11 +992,16 @@ int rsdf_class_head_fwd(const void *x, const void *w, int64_t n, int64_t v, int 
     RSDF_CHECK_ARG(s.at <= workspace_bytes, "class_head_fwd: workspace too small");
     hipStream_t st = (hipStream_t)stream;
     const int64_t xplane = p.n_pad * p.dp, wplane = p.vf * p.dp;
-    if (!p.direct) pack(dtype, x, n, d, p.n_pad, p.dp, nullptr, f.xp, st);
     for (int64_t v0 = 0; v0 < v; v0 += p.vf) {
         const int64_t here = v - v0 < p.vf ? v - v0 : p.vf;
         HeadArgs a = {};
-        if (!p.direct) pack(dtype, row_ptr(w, v0, d, dtype), here, d, p.vf, p.dp, nullptr, f.wp, st);
+        if (!p.direct) {
+            PrepArgs r = {};
+            r.d = d; r.dp = p.dp; r.wide = d % (dtype == T_F32 ? 4 : 8) == 0;
+            if (v0 == 0) add_pack(r, 0, x, n, p.n_pad, f.xp);
+            add_pack(r, 1, row_ptr(w, v0, d, dtype), here, p.vf, f.wp);
+            prep(dtype, r, st);
+        }
         a.x = p.direct ? rows_of(x, 0, d) : rows_of(f.xp, xplane, p.dp);
         a.w = p.direct ? rows_of(row_ptr(w, v0, d, dtype), 0, d) : rows_of(f.wp, wplane, p.dp);
         a.n = n; a.vc = here;
@@ -844,15 +1009,12 @@ int rsdf_class_head_fwd(const void *x, const void *w, int64_t n, int64_t v, int 
         a.depth = p.dp;
         a.c = LOG2E / temperature;
         a.stats = f.stats;
-        a.tile0 = v0 / 256;
+        a.tile0 = v0 / p.sbm;
         head<false>(p, a, st);
     }
-    RowArgs r = {x, w, n, v, d, k, f.stats, up(v, 256) / 256, ids, teacher_logits, ignore_id, temperature,
+    RowArgs r = {x, w, n, v, d, k, f.stats, (v + p.sbm - 1) / p.sbm, ids, teacher_logits, ignore_id, temperature,
                  reduction == 0 ? loss : f.loss, lse, q, listed_z, bad_ids};
-    const unsigned g = (unsigned)((n + 3) / 4);
-    if (dtype == T_F32) rows_kernel<T_F32><<<g, 256, 0, st>>>(r);
-    else if (dtype == T_BF16) rows_kernel<T_BF16><<<g, 256, 0, st>>>(r);
-    else rows_kernel<T_F16><<<g, 256, 0, st>>>(r);
+    rows_pass(dtype, r, st);
     if (reduction != 0) sum_kernel<<<1, 1024, 0, st>>>(f.loss, lse, n, reduction == 1, loss, count);
     RSDF_RETURN_LAUNCH();
 }
@@ -875,14 +1037,22 @@ int rsdf_class_head_bwd(const void *x, const void *w, int64_t n, int64_t v, int 
     const int nseg = p.parts == 3 ? 6 : 1;
     const int64_t xplane = p.n_pad * p.dp, wplane = p.vc * p.dp, zplane = p.n_pad * p.vc;
     const float scale = dtype == T_F16 ? 1.0f / F16_DZ : 1.0f;
-    weights_kernel<<<1, 1024, 0, st>>>(lse, grad, grad_per_row, count, temperature, n, b.weight, b.top);
-    if (!p.direct) pack(dtype, x, n, d, p.n_pad, p.dp, nullptr, b.xp, st);
-    if (dw != nullptr) pack(dtype, x, n, d, p.n_pad, p.dp, b.weight, b.xs, st);
     for (int64_t v0 = 0; v0 < v; v0 += p.vc) {
         const int64_t here = v - v0 < p.vc ? v - v0 : p.vc;
         HeadArgs a = {};
-        if (!p.direct) pack(dtype, row_ptr(w, v0, d, dtype), here, d, p.vc, p.dp, nullptr, b.wp, st);
-        a.x = p.direct ? rows_of(x, 0, d) : rows_of(b.xp, xplane, p.dp);
+        if (v0 == 0 || !p.direct) {
+            PrepArgs r = {};
+            r.d = d; r.dp = p.dp; r.wide = d % (dtype == T_F32 ? 4 : 8) == 0;
+            if (v0 == 0) {
+                r.lse = lse; r.g = grad; r.count = count; r.g_per_row = grad_per_row;
+                r.temperature = temperature; r.n = n;
+                r.weight = b.weight; r.top = b.top;
+                if (b.xs != nullptr) add_pack(r, 0, x, n, p.n_pad, b.xs);
+            }
+            if (!p.direct) add_pack(r, 1, row_ptr(w, v0, d, dtype), here, p.vc, b.wp);
+            prep(dtype, r, st);
+        }
+        a.x = p.direct ? rows_of(x, 0, d) : rows_of(b.xs, xplane, p.dp);
         a.w = p.direct ? rows_of(row_ptr(w, v0, d, dtype), 0, d) : rows_of(b.wp, wplane, p.dp);
         a.n = n; a.n_pad = p.n_pad; a.vc = here; a.ldz = p.vc;
         a.nseg = nseg;
@@ -895,7 +1065,7 @@ int rsdf_class_head_bwd(const void *x, const void *w, int64_t n, int64_t v, int 
         a.dz = b.dz;
         head<true>(p, a, st);
         if (q != nullptr) {
-            const unsigned g = (unsigned)((n * k + 255) / 256);
+            const unsigned g = (unsigned)((n + 3) / 4);
             if (dtype == T_F32) listed_kernel<false, 3><<<g, 256, 0, st>>>(ids, q, listed_z, lse, b.weight, b.top, n, k, a.c, v0, p.vc, p.n_pad, b.dz);
             else if (dtype == T_BF16) listed_kernel<false, 1><<<g, 256, 0, st>>>(ids, q, listed_z, lse, b.weight, b.top, n, k, a.c, v0, p.vc, p.n_pad, b.dz);
             else listed_kernel<true, 1><<<g, 256, 0, st>>>(ids, q, listed_z, lse, b.weight, b.top, n, k, a.c, v0, p.vc, p.n_pad, b.dz);
@@ -925,9 +1095,11 @@ int rsdf_class_head_bwd(const void *x, const void *w, int64_t n, int64_t v, int 
             pw.scale = scale;
         }
         products(p, pw, px, st);
-        if (b.dwp != nullptr) join(p, b.dwp, pw.part_stride, p.split_dw, here, nullptr, b.top, scale, pw.out, st);
+        Join ja = {}, jb = {};
+        if (b.dwp != nullptr) ja = Join{b.dwp, pw.part_stride, here, p.split_dw, nullptr, pw.out};
+        if (dx != nullptr && v0 + p.vc >= v) jb = Join{b.dxp, n * p.dp, n, p.split_dx, b.weight, dx};
+        join(p, ja, jb, b.top, scale, st);
     }
-    if (dx != nullptr) join(p, b.dxp, n * p.dp, p.split_dx, n, b.weight, b.top, scale, dx, st);
     RSDF_RETURN_LAUNCH();
 }
 

@@ -6,7 +6,7 @@
 // Both are bound by memory: the lookup reads each row that occurs and writes N rows, the gradient reads N rows and writes V.
 // Products and sums are fp32, one rounding to the table's type at the end.
 //
-// The gradient sorts the positions by id (a stable radix sort of at most 8 bits a pass) and sums the rows of one id in
+// The gradient sorts the positions by id (a stable radix sort) and sums the rows of one id in
 // order: no float atomics, the same bits every time.  The sorted list is cut into chunks of equal LENGTH, so an id that takes
 // half of all positions costs no more than any other: a group of lanes sums its chunk's runs; a run that lies inside one chunk
 // is written at once, one that crosses chunks leaves its parts in `part` for the join.  Rows of the table that no position
@@ -17,6 +17,7 @@
 namespace {
 
 constexpr int T_F32 = 0, T_BF16 = 1, T_F16 = 2;
+constexpr int64_t L2_BYTES = 32ll << 20;          // of the eight XCDs
 
 template <int DT> struct Elem;
 template <> struct Elem<T_F32> {
@@ -36,37 +37,70 @@ template <> struct Elem<T_F16> {
 };
 template <class T, int N> struct alignas(sizeof(T) * N) Vec { T v[N]; };
 
+// a store that does not stay in the caches: written once, read by someone else
+template <class V>
+__device__ __forceinline__ void nt_store(V *p, const V &v)
+{
+    if constexpr (sizeof(V) == 16) {
+        using B = __attribute__((ext_vector_type(4))) unsigned;
+        __builtin_nontemporal_store(*(const B *)&v, (B *)p);
+    } else if constexpr (sizeof(V) == 8) {
+        using B = __attribute__((ext_vector_type(2))) unsigned;
+        __builtin_nontemporal_store(*(const B *)&v, (B *)p);
+    } else {
+        *p = v;
+    }
+}
+
 // ---- lookup -------------------------------------------------------------------------------------------------------------------
-template <int DT, int VW>
+// NT: the output passes the caches by (262144 x 256 bf16: 28 instead of 42 us, and the table stays in them)
+template <int DT, int VW, bool NT>
 __global__ void __launch_bounds__(256) lookup_kernel(const int64_t *__restrict__ ids, int64_t n, const void *__restrict__ table, int64_t v,
                                                      int per_row, float scale, int64_t padding, int rows_per_block,
                                                      void *__restrict__ out, int *__restrict__ bad_ids)
 {
     using E = Elem<DT>;
     using V = Vec<typename E::type, VW>;
+    constexpr int U = 4;
     const int64_t r0 = (int64_t)blockIdx.x * rows_per_block;
-    const int rows = (int)(n - r0 < rows_per_block ? n - r0 : rows_per_block);
-    for (int i = threadIdx.x; i < rows * per_row; i += 256) {
-        const int r = i / per_row, c = i - r * per_row;
-        const int64_t id = ids[r0 + r];
-        V o;
-        if (id >= 0 && id < v && id != padding) {
-            const V t = ((const V *)table)[id * per_row + c];
+    const int rows = (int)(n - r0 < rows_per_block ? n - r0 : rows_per_block), items = rows * per_row;
+    for (int i0 = threadIdx.x; i0 < items; i0 += 256 * U) {
+        int64_t id[U];
+        int c[U];
+        V o[U];
 #pragma unroll
-            for (int e = 0; e < VW; ++e) o.v[e] = E::put(E::get(t.v[e]) * scale);
-        } else {
-            const float f = id == padding ? 0.0f : __builtin_nanf("");
-#pragma unroll
-            for (int e = 0; e < VW; ++e) o.v[e] = E::put(f);
-            if (c == 0 && id != padding && bad_ids != nullptr) atomicAdd(bad_ids, 1);
+        for (int u = 0; u < U; ++u) {
+            const int i = i0 + u * 256 < items ? i0 + u * 256 : i0;
+            const int r = i / per_row;
+            c[u] = i - r * per_row;
+            id[u] = ids[r0 + r];
         }
-        ((V *)out)[(r0 + r) * per_row + c] = o;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const bool in = id[u] >= 0 && id[u] < v;
+            o[u] = ((const V *)table)[(in ? id[u] : 0) * per_row + c[u]];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (i0 + u * 256 >= items) continue;
+            const bool in = id[u] >= 0 && id[u] < v;
+#pragma unroll
+            for (int e = 0; e < VW; ++e) {
+                const float f = in ? E::get(o[u].v[e]) * scale : __builtin_nanf("");
+                o[u].v[e] = E::put(id[u] == padding ? 0.0f : f);
+            }
+            if (!in && id[u] != padding && c[u] == 0 && bad_ids != nullptr) atomicAdd(bad_ids, 1);
+            if (NT) nt_store((V *)out + r0 * per_row + i0 + u * 256, o[u]);
+            else ((V *)out)[r0 * per_row + i0 + u * 256] = o[u];
+        }
     }
 }
 
 // ---- stable radix sort of (id, position) ----------------------------------------------------------------------------------------
-// One pass = a histogram per workgroup and a scatter; a workgroup's share is contiguous, at most MAX_BLOCKS workgroups.
-constexpr int SORT_BINS = 256, MAX_BLOCKS = 256, SORT_ROUND = 256;
+// A pass: a histogram per workgroup (left out where there is one workgroup) and a scatter.  A workgroup's share of the list is
+// contiguous and so is a wave's part of it: a wave ranks its 64 x ITEMS items among themselves with ballots, one table of counts per
+// wave in LDS, and the waves' tables are summed once.  Up to 9 bits a pass: two passes for 2^18 ids.
+constexpr int SORT_THREADS = 512, SORT_WAVES = 8, ITEMS = 4, ROUND = SORT_THREADS * ITEMS, SORT_BITS = 9, BINS = 1 << SORT_BITS, MAX_BLOCKS = 128;
 
 __device__ __forceinline__ unsigned sort_key(const int64_t *ids, const unsigned *keys, int64_t i, int64_t v, int64_t padding)
 {
@@ -75,7 +109,7 @@ __device__ __forceinline__ unsigned sort_key(const int64_t *ids, const unsigned 
     return (id >= 0 && id < v && id != padding) ? (unsigned)id : (unsigned)v;      // v: behind every real id
 }
 
-// lanes of this wave with the same digit as this lane (among the lanes in `active`)
+// lanes of this wave in `active` with the same digit as this lane
 __device__ __forceinline__ unsigned long long same_digit(unsigned digit, int bits, unsigned long long active)
 {
     unsigned long long m = active;
@@ -86,65 +120,141 @@ __device__ __forceinline__ unsigned long long same_digit(unsigned digit, int bit
     return m;
 }
 
-__global__ void __launch_bounds__(256) sort_count_kernel(const int64_t *__restrict__ ids, const unsigned *__restrict__ keys, int64_t n, int64_t v,
-                                                         int64_t padding, int shift, int bits, int64_t share, unsigned *__restrict__ counts)
+__global__ void __launch_bounds__(SORT_THREADS) sort_count_kernel(const int64_t *__restrict__ ids, const unsigned *__restrict__ keys, int64_t n,
+                                                                  int64_t v, int64_t padding, int shift, int bits, int64_t share,
+                                                                  unsigned *__restrict__ counts)
 {
-    __shared__ unsigned c[SORT_BINS];
+    __shared__ unsigned c[BINS];
     c[threadIdx.x] = 0;
     __syncthreads();
     const int64_t b = blockIdx.x * share, e = b + share < n ? b + share : n;
     const unsigned mask = (1u << bits) - 1;
-    for (int64_t i = b + threadIdx.x; i < e; i += 256) atomicAdd(&c[(sort_key(ids, keys, i, v, padding) >> shift) & mask], 1u);
+#pragma unroll 4
+    for (int64_t i = b + threadIdx.x; i < e; i += SORT_THREADS) atomicAdd(&c[(sort_key(ids, keys, i, v, padding) >> shift) & mask], 1u);
     __syncthreads();
-    counts[blockIdx.x * SORT_BINS + threadIdx.x] = c[threadIdx.x];
+    counts[blockIdx.x * BINS + threadIdx.x] = c[threadIdx.x];
 }
 
-__global__ void __launch_bounds__(256) sort_scatter_kernel(const int64_t *__restrict__ ids, const unsigned *__restrict__ keys,
-                                                           const unsigned *__restrict__ pos, int64_t n, int64_t v, int64_t padding, int shift,
-                                                           int bits, int64_t share, const unsigned *__restrict__ counts,
-                                                           unsigned *__restrict__ keys_out, unsigned *__restrict__ pos_out)
+__global__ void __launch_bounds__(SORT_THREADS) sort_scatter_kernel(const int64_t *__restrict__ ids, const unsigned *__restrict__ keys,
+                                                                    const unsigned *__restrict__ pos, int64_t n, int64_t v, int64_t padding,
+                                                                    int shift, int bits, int64_t share, const unsigned *__restrict__ counts,
+                                                                    unsigned *__restrict__ keys_out, unsigned *__restrict__ pos_out)
 {
-    __shared__ unsigned base[SORT_BINS];               // where this workgroup's next item of a digit goes
-    __shared__ unsigned wave_count[4][SORT_BINS];
-    __shared__ unsigned total[4];
+    __shared__ unsigned count[SORT_WAVES][BINS];       // items of a digit in a wave's part, then where its next one goes
+    __shared__ unsigned total[SORT_WAVES];
     const int t = threadIdx.x, lane = t & 63, w = t >> 6;
-    // items of smaller digits anywhere + items of this digit in earlier workgroups
-    unsigned before = 0, all = 0;
-    for (int b = 0; b < (int)gridDim.x; ++b) {
-        const unsigned c = counts[b * SORT_BINS + t];
-        before += b < (int)blockIdx.x ? c : 0;
-        all += c;
-    }
-    unsigned incl = (unsigned)wave_incl_sum_i((int)all);
-    if (lane == 63) total[w] = incl;
-    __syncthreads();
-    for (int k = 0; k < w; ++k) incl += total[k];
-    base[t] = incl - all + before;
-    const int64_t b0 = blockIdx.x * share, e0 = b0 + share < n ? b0 + share : n;
     const unsigned mask = (1u << bits) - 1;
-    for (int64_t r = b0; r < e0; r += SORT_ROUND) {
-        for (int k = 0; k < 4; ++k) wave_count[k][t] = 0;
+    // sum over the digits before digit t of their items
+    auto before_digit = [&](unsigned all) {
+        unsigned incl = (unsigned)wave_incl_sum_i((int)all);
+        if (lane == 63) total[w] = incl;
         __syncthreads();
-        const int64_t i = r + t;
-        const bool here = i < e0;
-        const unsigned key = here ? sort_key(ids, keys, i, v, padding) : 0;
-        const unsigned digit = (key >> shift) & mask;
-        const unsigned long long same = same_digit(digit, bits, __ballot(here));
-        const unsigned rank = __popcll(same & ((1ull << lane) - 1));
-        if (here && rank == 0) wave_count[w][digit] = (unsigned)__popcll(same);
+        for (int k = 0; k < w; ++k) incl += total[k];
+        return incl - all;
+    };
+    unsigned base = 0;                                 // where the next item of digit t goes
+    if (gridDim.x > 1) {
+        unsigned before = 0, all = 0;
+#pragma unroll 16
+        for (int b = 0; b < (int)gridDim.x; ++b) {
+            const unsigned c = counts[b * BINS + t];
+            before += b < (int)blockIdx.x ? c : 0;
+            all += c;
+        }
+        base = before_digit(all) + before;
+    }
+    const int64_t b0 = blockIdx.x * share, e0 = b0 + share < n ? b0 + share : n;
+    for (int64_t r = b0; r < e0; r += ROUND) {
+        const int64_t first = r + w * (64 * ITEMS) + lane;
+        unsigned key[ITEMS], rank[ITEMS];
+#pragma unroll
+        for (int j = 0; j < ITEMS; ++j) key[j] = first + j * 64 < e0 ? sort_key(ids, keys, first + j * 64, v, padding) : 0;
+        for (int k = lane; k < BINS; k += 64) count[w][k] = 0;
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int j = 0; j < ITEMS; ++j) {
+            const bool here = first + j * 64 < e0;
+            const unsigned digit = (key[j] >> shift) & mask;
+            const unsigned long long same = same_digit(digit, bits, __ballot(here));
+            const unsigned mine = __popcll(same & ((1ull << lane) - 1));
+            volatile unsigned *c = &count[w][digit];
+            const unsigned seen = *c;
+            rank[j] = seen + mine;
+            if (here && mine == 0) *c = seen + (unsigned)__popcll(same);
+            __builtin_amdgcn_wave_barrier();
+        }
         __syncthreads();
-        if (here) {
-            unsigned at = base[digit] + rank;
-            for (int k = 0; k < w; ++k) at += wave_count[k][digit];
-            keys_out[at] = key;
+        unsigned all = 0;
+        for (int k = 0; k < SORT_WAVES; ++k) {
+            const unsigned c = count[k][t];
+            count[k][t] = all;
+            all += c;
+        }
+        if (gridDim.x == 1 && r == b0 && e0 - b0 <= ROUND) base = before_digit(all);       // the whole list is here
+        for (int k = 0; k < SORT_WAVES; ++k) count[k][t] += base;
+        base += all;
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < ITEMS; ++j) {
+            const int64_t i = first + j * 64;
+            if (i >= e0) continue;
+            const unsigned at = count[w][(key[j] >> shift) & mask] + rank[j];
+            keys_out[at] = key[j];
             pos_out[at] = pos == nullptr ? (unsigned)i : pos[i];
         }
         __syncthreads();
-        base[t] += wave_count[0][t] + wave_count[1][t] + wave_count[2][t] + wave_count[3][t];
+    }
+}
+
+// ---- few positions: no list -----------------------------------------------------------------------------------------------------
+// One wave per row of the table walks all ids, 64 at a time, and adds up its positions in order: one launch, no workspace.
+template <int DT, int VW>
+__global__ void __launch_bounds__(256) few_kernel(const int64_t *__restrict__ ids, int n, const void *__restrict__ g, int64_t v, int per_row,
+                                                  float scale, int64_t padding, void *__restrict__ out)
+{
+    using E = Elem<DT>;
+    using V = Vec<typename E::type, VW>;
+    const int lane = threadIdx.x & 63;
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= v) return;
+    for (int c = lane; c - lane < per_row; c += 64) {
+        float acc[VW];
+#pragma unroll
+        for (int k = 0; k < VW; ++k) acc[k] = 0.0f;
+        for (int i0 = 0; i0 < n; i0 += 64) {
+            const bool mine = i0 + lane < n && ids[i0 + lane] == row && row != padding;
+            unsigned long long m = __ballot(mine);
+            while (m != 0) {
+                constexpr int U = 8;                     // rows on their way at once
+                V x[U];
+                int here = 0;
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    if (m == 0) continue;
+                    const int at = i0 + __ffsll((long long)m) - 1;
+                    m &= m - 1;
+                    here = u + 1;
+                    x[u] = ((const V *)g)[(int64_t)at * per_row + (c < per_row ? c : 0)];
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    if (u >= here) continue;
+#pragma unroll
+                    for (int k = 0; k < VW; ++k) acc[k] += E::get(x[u].v[k]);
+                }
+            }
+        }
+        if (c < per_row) {
+            V o;
+#pragma unroll
+            for (int k = 0; k < VW; ++k) o.v[k] = E::put(acc[k] * scale);
+            ((V *)out)[row * per_row + c] = o;
+        }
     }
 }
 
 // ---- sums over the sorted list --------------------------------------------------------------------------------------------------
+constexpr int LONG = 16;         // a run over more chunks than this is joined by a whole workgroup
 struct SumArgs {
     const unsigned *keys, *pos;
     int64_t n, v;
@@ -154,6 +264,7 @@ struct SumArgs {
     const void *g;
     float scale;
     float *part;                 // [chunk][2][d]: what continues a run of earlier chunks; what begins a run that goes on
+    unsigned char *goes_on;      // [chunk]: a run begins there that goes on (1; 2 over more than LONG chunks)
     void *out;
     int64_t sum_blocks;          // later workgroups zero rows
     int zero_rows;               // rows per such workgroup
@@ -198,7 +309,7 @@ __global__ void __launch_bounds__(256) sum_kernel(SumArgs a)
     const unsigned none = (unsigned)a.v;
     const unsigned prev = b > 0 ? a.keys[b - 1] : none, next = e < a.n ? a.keys[e] : none;
     unsigned cur = a.keys[b];
-    bool first = true;
+    bool first = true, marked = false;
     float acc[VW];
 #pragma unroll
     for (int k = 0; k < VW; ++k) acc[k] = 0.0f;
@@ -214,6 +325,11 @@ __global__ void __launch_bounds__(256) sum_kernel(SumArgs a)
             float *p = a.part + (c * 2 + (head ? 0 : 1)) * a.d + col * VW;
 #pragma unroll
             for (int k = 0; k < VW; ++k) p[k] = acc[k];
+            if (!head && col == 0) {
+                const int64_t far = b + (int64_t)a.chunk * (LONG + 1);
+                a.goes_on[c] = far < a.n && a.keys[far] == cur ? 2 : 1;
+                marked = true;
+            }
         }
     };
     for (int64_t i = b; i < e; i += U) {
@@ -240,38 +356,66 @@ __global__ void __launch_bounds__(256) sum_kernel(SumArgs a)
         }
     }
     flush(true);
+    if (!marked && col == 0) a.goes_on[c] = 0;
 }
 
-// a run that begins in chunk c and goes on: its parts in order, 4 waves taking every fourth part
+// The runs that cross chunks: one wave per chunk and 64 columns looks whether one begins there.  A short run it joins by itself, a
+// long one with the other 15 waves of the workgroup (each every sixteenth part).
+constexpr int JOIN_WAVES = 16;
 template <int DT>
-__global__ void __launch_bounds__(256) join_kernel(SumArgs a)
+__global__ void __launch_bounds__(64 * JOIN_WAVES) join_kernel(SumArgs a)
 {
     using E = Elem<DT>;
-    __shared__ float sums[4][64];
-    const int64_t c = blockIdx.x, b = c * a.chunk, e = b + a.chunk;
-    if (e >= a.n) return;
-    const unsigned key = a.keys[e - 1];
-    if (key == (unsigned)a.v || a.keys[e] != key) return;
-    if (b > 0 && a.keys[b] == key && a.keys[b - 1] == key) return;      // began earlier
-    int64_t lo = e, hi = a.n;                                           // first position behind the run
-    while (lo < hi) {
-        const int64_t mid = (lo + hi) >> 1;
-        if (a.keys[mid] <= key) lo = mid + 1;
-        else hi = mid;
+    using T = typename E::type;
+    __shared__ float sums[JOIN_WAVES][64];
+    __shared__ unsigned char is_long[JOIN_WAVES];
+    const int segs = (a.d + 63) / 64, l = threadIdx.x & 63, w = threadIdx.x >> 6;
+    // (chunks run fastest: the columns of one long run go to different workgroups)
+    const int64_t job0 = (int64_t)blockIdx.x * JOIN_WAVES, each = a.chunks - 1, jobs = each * segs;
+    const int kind = job0 + w < jobs ? a.goes_on[(job0 + w) % each] : 0;
+    if (l == 0) is_long[w] = kind == 2;
+    if (kind == 1) {
+        const int64_t c = (job0 + w) % each, e = (c + 1) * a.chunk;
+        const unsigned key = a.keys[e];
+        // chunks behind c that begin with this id (at most LONG)
+        const int64_t at = e + (int64_t)l * a.chunk;
+        const unsigned long long other = ~__ballot(at < a.n && a.keys[at] == key);
+        const int parts = __ffsll((long long)other) - 1;
+        const int col = (int)((job0 + w) / each) * 64 + l;
+        if (col < a.d) {
+            float s = a.part[(c * 2 + 1) * a.d + col];
+#pragma unroll 4
+            for (int k = 1; k <= parts; ++k) s += a.part[(c + k) * 2 * a.d + col];
+            ((T *)a.out)[(int64_t)key * a.d + col] = E::put(s * a.scale);
+        }
     }
-    const int64_t last = (lo - 1) / a.chunk;
-    const int w = threadIdx.x >> 6, col = blockIdx.y * 64 + (threadIdx.x & 63);
-    float s = 0.0f;
-    if (col < a.d) {
-        if (w == 0) s = a.part[(c * 2 + 1) * a.d + col];
-        for (int64_t k = c + 1 + w; k <= last; k += 4) s += a.part[k * 2 * a.d + col];
-    }
-    sums[w][threadIdx.x & 63] = s;
     __syncthreads();
-    if (w == 0 && col < a.d) {
-        const int l = threadIdx.x;
-        s = (sums[0][l] + sums[1][l]) + (sums[2][l] + sums[3][l]);
-        ((typename E::type *)a.out)[(int64_t)key * a.d + col] = E::put(s * a.scale);
+    for (int i = 0; i < JOIN_WAVES; ++i) {
+        if (!is_long[i]) continue;
+        const int64_t c = (job0 + i) % each, e = (c + 1) * a.chunk;
+        const unsigned key = a.keys[e];
+        int64_t last = c;                                               // the last chunk that begins with this id
+        for (int here = JOIN_WAVES * 64; here == JOIN_WAVES * 64;) {
+            const int64_t at = (last + 1 + threadIdx.x) * a.chunk;
+            here = __syncthreads_count(at < a.n && a.keys[at] == key);
+            last += here;
+        }
+        const int col = (int)((job0 + i) / each) * 64 + l;
+        float s = 0.0f;
+        if (col < a.d) {
+            if (w == 0) s = a.part[(c * 2 + 1) * a.d + col];
+#pragma unroll 4
+            for (int64_t k = c + 1 + w; k <= last; k += JOIN_WAVES) s += a.part[k * 2 * a.d + col];
+        }
+        sums[w][l] = s;
+        __syncthreads();
+        if (w == 0 && col < a.d) {
+            s = 0.0f;
+#pragma unroll
+            for (int k = 0; k < JOIN_WAVES; ++k) s += sums[k][l];
+            ((T *)a.out)[(int64_t)key * a.d + col] = E::put(s * a.scale);
+        }
+        __syncthreads();
     }
 }
 
@@ -283,17 +427,19 @@ Sorting sorting(int64_t n, int64_t v)
     int bits = 1;
     while ((1ll << bits) <= v) ++bits;           // keys 0 .. v
     Sorting s;
-    s.passes = (bits + 7) / 8;
+    s.passes = (bits + SORT_BITS - 1) / SORT_BITS;
     s.bits = (bits + s.passes - 1) / s.passes;
-    s.share = up((n + MAX_BLOCKS - 1) / MAX_BLOCKS, SORT_ROUND);
-    s.share = s.share < 1024 ? 1024 : s.share;
+    s.share = up((n + MAX_BLOCKS - 1) / MAX_BLOCKS, ROUND);
     s.blocks = (unsigned)((n + s.share - 1) / s.share);
     return s;
 }
 
-int chunk_of(int64_t n) { const int64_t c = n / 4096; return (int)(c < 8 ? 8 : (c > 64 ? 64 : c)); }
+int chunk_of(int64_t n) { const int64_t c = n / 8192; return (int)(c < 8 ? 8 : (c > 64 ? 64 : c)); }
 
-struct Space { unsigned *keys[2], *pos[2], *counts; float *part; int64_t bytes; };
+// Walking all ids per row of the table instead of sorting them: n / 64 steps for each of v waves, and every addition of a row in turn
+bool use_few(int64_t n, int64_t v) { return n > 0 && n <= 512 && n * v <= (1 << 23); }
+
+struct Space { unsigned *keys[2], *pos[2], *counts; unsigned char *goes_on; float *part; int64_t bytes; };
 Space space(void *ws, int64_t n, int64_t v, int d)
 {
     Space s;
@@ -304,8 +450,9 @@ Space space(void *ws, int64_t n, int64_t v, int d)
         return p;
     };
     for (int i = 0; i < 2; ++i) { s.keys[i] = (unsigned *)take(n * 4); s.pos[i] = (unsigned *)take(n * 4); }
-    s.counts = (unsigned *)take(MAX_BLOCKS * SORT_BINS * 4);
+    s.counts = (unsigned *)take(MAX_BLOCKS * BINS * 4);
     const int64_t chunk = chunk_of(n);
+    s.goes_on = (unsigned char *)take((n + chunk - 1) / chunk);
     s.part = (float *)take((n + chunk - 1) / chunk * 2 * d * 4);
     s.bytes = at;
     return s;
@@ -362,7 +509,10 @@ int rsdf_embedding_fwd(const int64_t *ids, int64_t n, const void *table, int64_t
     int rows = 1024 / per_row;                          // about four vectors a thread
     rows = rows < 1 ? 1 : rows;
     const unsigned grid = (unsigned)((n + rows - 1) / rows);
-#define CALL(DT, VW) lookup_kernel<DT, VW><<<grid, 256, 0, (hipStream_t)stream>>>(ids, n, table, v, per_row, scale, padding_id, rows, out, bad_ids)
+    const bool past = n * d * (dtype == T_F32 ? 4 : 2) >= L2_BYTES;
+#define CALL(DT, VW)                                                                                                                   \
+    past ? lookup_kernel<DT, VW, true><<<grid, 256, 0, (hipStream_t)stream>>>(ids, n, table, v, per_row, scale, padding_id, rows, out, bad_ids) \
+         : lookup_kernel<DT, VW, false><<<grid, 256, 0, (hipStream_t)stream>>>(ids, n, table, v, per_row, scale, padding_id, rows, out, bad_ids)
     RSDF_EMBEDDING_DISPATCH(dtype, bytes, CALL);
 #undef CALL
     RSDF_RETURN_LAUNCH();
@@ -372,7 +522,7 @@ int64_t rsdf_embedding_bwd_workspace_bytes(int64_t n, int64_t v, int d)
 {
     const char *bad = bad_shape(n, v, d, T_F32);
     if (bad != nullptr) { rsdf_set_error(bad); return -1; }
-    return space(nullptr, n, v, d).bytes;
+    return use_few(n, v) ? 0 : space(nullptr, n, v, d).bytes;
 }
 
 int rsdf_embedding_bwd(const int64_t *ids, int64_t n, const void *grad, int64_t v, int d, int dtype, float scale, int64_t padding_id,
@@ -380,28 +530,36 @@ int rsdf_embedding_bwd(const int64_t *ids, int64_t n, const void *grad, int64_t 
 {
     const char *bad = bad_shape(n, v, d, dtype);
     RSDF_CHECK_ARG(bad == nullptr, bad);
+    hipStream_t st = (hipStream_t)stream;
+    const int bytes = vector_bytes(d, dtype, grad, d_table);
+    const int per_row = d * (dtype == T_F32 ? 4 : 2) / bytes;
+    if (use_few(n, v)) {
+#define CALL(DT, VW) few_kernel<DT, VW><<<(unsigned)((v + 3) / 4), 256, 0, st>>>(ids, (int)n, grad, v, per_row, scale, padding_id, d_table)
+        RSDF_EMBEDDING_DISPATCH(dtype, bytes, CALL);
+#undef CALL
+        RSDF_RETURN_LAUNCH();
+    }
     const Space s = space(workspace, n, v, d);
     RSDF_CHECK_ARG(s.bytes <= workspace_bytes, "embedding_bwd: workspace too small");
-    hipStream_t st = (hipStream_t)stream;
     const Sorting so = sorting(n, v);
     int from = 1;
     if (n > 0)
         for (int p = 0; p < so.passes; ++p) {
             const int64_t *first = p == 0 ? ids : nullptr;
             const int to = 1 - from;
-            sort_count_kernel<<<so.blocks, 256, 0, st>>>(first, s.keys[from], n, v, padding_id, p * so.bits, so.bits, so.share, s.counts);
-            sort_scatter_kernel<<<so.blocks, 256, 0, st>>>(first, s.keys[from], p == 0 ? nullptr : s.pos[from], n, v, padding_id,
-                                                           p * so.bits, so.bits, so.share, s.counts, s.keys[to], s.pos[to]);
+            if (so.blocks > 1)
+                sort_count_kernel<<<so.blocks, SORT_THREADS, 0, st>>>(first, s.keys[from], n, v, padding_id, p * so.bits, so.bits, so.share,
+                                                                      s.counts);
+            sort_scatter_kernel<<<so.blocks, SORT_THREADS, 0, st>>>(first, s.keys[from], p == 0 ? nullptr : s.pos[from], n, v, padding_id,
+                                                                    p * so.bits, so.bits, so.share, s.counts, s.keys[to], s.pos[to]);
             from = to;
         }
-    const int bytes = vector_bytes(d, dtype, grad, d_table);
-    const int per_row = d * (dtype == T_F32 ? 4 : 2) / bytes;
     SumArgs a;
     a.keys = s.keys[from]; a.pos = s.pos[from];
     a.n = n; a.v = v; a.d = d; a.per_row = per_row;
     a.chunk = chunk_of(n);
     a.chunks = (n + a.chunk - 1) / a.chunk;
-    a.g = grad; a.scale = scale; a.part = s.part; a.out = d_table;
+    a.g = grad; a.scale = scale; a.part = s.part; a.goes_on = s.goes_on; a.out = d_table;
     a.lanes = 1;
     while (a.lanes < per_row && a.lanes < 64) a.lanes *= 2;
     a.groups = 256 / a.lanes;
@@ -414,10 +572,11 @@ int rsdf_embedding_bwd(const int64_t *ids, int64_t n, const void *grad, int64_t 
     RSDF_EMBEDDING_DISPATCH(dtype, bytes, CALL);
 #undef CALL
     if (a.chunks > 1) {
-        const dim3 g((unsigned)(a.chunks - 1), (unsigned)((d + 63) / 64));
-        if (dtype == T_F32) join_kernel<T_F32><<<g, 256, 0, st>>>(a);
-        else if (dtype == T_BF16) join_kernel<T_BF16><<<g, 256, 0, st>>>(a);
-        else join_kernel<T_F16><<<g, 256, 0, st>>>(a);
+        const int64_t jobs = (a.chunks - 1) * ((d + 63) / 64);
+        const unsigned g = (unsigned)((jobs + JOIN_WAVES - 1) / JOIN_WAVES);
+        if (dtype == T_F32) join_kernel<T_F32><<<g, 64 * JOIN_WAVES, 0, st>>>(a);
+        else if (dtype == T_BF16) join_kernel<T_BF16><<<g, 64 * JOIN_WAVES, 0, st>>>(a);
+        else join_kernel<T_F16><<<g, 64 * JOIN_WAVES, 0, st>>>(a);
     }
     RSDF_RETURN_LAUNCH();
 }

@@ -14,6 +14,7 @@ import torch
 
 from . import _lib as L
 from ._lib import check, lib, ptr, require_device, stream_ptr
+from .ops import DTYPE_IDS, _dtype_id, _int_ids, _same_device, once
 
 
 def _f(t):
@@ -128,86 +129,92 @@ _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 
 def _aligned(t):
     """Contiguous and 16-byte aligned (a view into the middle of a storage may be neither)."""
-    t = t.detach().contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+    if not t.is_contiguous():
+        return t.detach().contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.detach().clone()
+
+
+def _addr(t):
+    return None if t is None else t.data_ptr()
 
 
 class _ClassHead(torch.autograd.Function):
     """Both losses: ``logits`` None = labels (``ids`` [N, 1]), else a teacher's listed classes (``ids``, ``logits`` [N, K])."""
 
     @staticmethod
-    def forward(ctx, x, w, ids, logits, ignore, temperature, reduction):
-        from .ops import DTYPE_IDS
+    def forward(ctx, x, w, ids, logits, k, ignore, temperature, reduction):
         xc, wc = _aligned(x), _aligned(w)
-        require_device(xc, wc, ids, logits)
-        dev, (n, d), v, k = xc.device, xc.shape, wc.shape[0], ids.shape[1]
+        (n, d), v, device, l = xc.shape, wc.shape[0], xc.device, lib()
         dt = DTYPE_IDS[xc.dtype]
-        with torch.cuda.device(dev):
-            def f32(*shape):
-                return torch.empty(shape, dtype=torch.float32, device=dev)
-            nbytes = int(lib().rsdf_class_head_workspace_bytes(n, v, d, dt, 0))
-            if nbytes < 0:
-                check(1, "class_head_workspace_bytes")
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-            loss, lse = f32(n) if reduction == 0 else f32(1), f32(n)
-            count = f32(1) if reduction else None
-            q, zt = (f32(n, k), f32(n, k)) if logits is not None else (None, None)
-            check(lib().rsdf_class_head_fwd(ptr(xc), ptr(wc), n, v, d, dt, ptr(ids), ptr(logits), k, ignore, temperature,
-                                            reduction, ptr(loss), ptr(lse), ptr(count), ptr(q), ptr(zt),
-                                            L.bad_ids_ptr(dev), ptr(ws), nbytes, stream_ptr()), "class_head_fwd")
-        ctx.save_for_backward(xc, wc, ids, q, zt, lse, count)
-        ctx.temperature, ctx.reduction = temperature, reduction
-        return loss if reduction == 0 else loss.reshape(())
+        nbytes = l.rsdf_class_head_workspace_bytes(n, v, d, dt, 0)
+        if nbytes < 0:
+            check(1, "class_head_workspace_bytes")
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        # lse [n], count [1], and for a teacher q, listed logits [n, k]: one allocation, kept for the backward
+        keep = torch.empty(n + 1 + (2 * n * k if logits is not None else 0), dtype=torch.float32, device=device)
+        loss = torch.empty(n if reduction == 0 else (), dtype=torch.float32, device=device)
+        a = keep.data_ptr()
+        q, zt = (a + 4 * (n + 1), a + 4 * (n + 1 + n * k)) if logits is not None else (None, None)
+        dev = xc.get_device()
+        L.launch(dev, l.rsdf_class_head_fwd, "class_head_fwd", xc.data_ptr(), wc.data_ptr(), n, v, d, dt, ids.data_ptr(),
+                 _addr(logits), k, ignore, temperature, reduction, loss.data_ptr(), a, a + 4 * n, q, zt, L.bad_ids_ptr(dev),
+                 ws.data_ptr(), nbytes)
+        ctx.save_for_backward(xc, wc, ids, keep)
+        ctx.state = k, temperature, reduction, logits is not None
+        return loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once
     def backward(ctx, g):
-        from .ops import DTYPE_IDS
-        xc, wc, ids, q, zt, lse, count = ctx.saved_tensors
+        xc, wc, ids, keep = ctx.saved_tensors
+        k, temperature, reduction, teacher = ctx.state
         need_x, need_w = ctx.needs_input_grad[:2]
         if not (need_x or need_w):
-            return (None,) * 7
-        dev, (n, d), v, k = xc.device, xc.shape, wc.shape[0], ids.shape[1]
+            return (None,) * 8
+        (n, d), v, l = xc.shape, wc.shape[0], lib()
         dt = DTYPE_IDS[xc.dtype]
-        g = g.detach().to(torch.float32).reshape(-1).contiguous()
-        with torch.cuda.device(dev):
-            dx = torch.empty_like(xc) if need_x else None
-            dw = torch.empty_like(wc) if need_w else None
-            nbytes = int(lib().rsdf_class_head_workspace_bytes(n, v, d, dt, int(need_x) + 2 * int(need_w)))
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-            check(lib().rsdf_class_head_bwd(ptr(xc), ptr(wc), n, v, d, dt, ptr(ids), ptr(q), ptr(zt), k, ctx.temperature,
-                                            ptr(lse), ptr(count) if ctx.reduction == 1 else None, ptr(g),
-                                            int(ctx.reduction == 0), ptr(dx), ptr(dw), ptr(ws), nbytes, stream_ptr()),
-                  "class_head_bwd")
-        return dx, dw, None, None, None, None, None
+        g = g if g.is_contiguous() else g.contiguous()
+        dx = torch.empty_like(xc) if need_x else None
+        dw = torch.empty_like(wc) if need_w else None
+        nbytes = l.rsdf_class_head_workspace_bytes(n, v, d, dt, int(need_x) + 2 * int(need_w))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=xc.device)
+        a = keep.data_ptr()
+        q, zt = (a + 4 * (n + 1), a + 4 * (n + 1 + n * k)) if teacher else (None, None)
+        L.launch(xc.get_device(), l.rsdf_class_head_bwd, "class_head_bwd", xc.data_ptr(), wc.data_ptr(), n, v, d, dt,
+                 ids.data_ptr(), q, zt, k, temperature, a, a + 4 * n if reduction == 1 else None, g.data_ptr(),
+                 int(reduction == 0), _addr(dx), _addr(dw), ws.data_ptr(), nbytes)
+        return dx, dw, None, None, None, None, None, None
 
 
 def _class_head(what, x, weight, ids, logits, ignore, temperature, reduction):
-    from .ops import _dtype_id, _int_ids, _same_device
     err = L.RiseSdfHipError
     if reduction not in _REDUCTIONS:
         raise err(f"{what}: reduction {reduction!r}: none, mean or sum")
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
         raise err(f"{what}: features [..., D] and class codes [V, D], not {tuple(x.shape)} and {tuple(weight.shape)}")
-    if weight.shape[0] < 1 or weight.shape[1] < 1:
+    v, d = weight.shape
+    if v < 1 or d < 1:
         raise err(f"{what}: the head needs at least one class and one feature")
     if x.dtype != weight.dtype:
         raise err(f"{what}: features and class codes of one type, not {x.dtype} and {weight.dtype}")
     _dtype_id(x, what)
     ids = _int_ids(ids, what)
-    tensors = (x, weight, ids) if logits is None else (x, weight, ids, logits)
-    _same_device(what, *tensors)
-    require_device(*(t.contiguous() for t in tensors))
+    if logits is not None:
+        logits = _f(logits)
+        _same_device(what, x, weight, ids, logits)
+    else:
+        _same_device(what, x, weight, ids)
+    if not x.is_cuda:
+        raise err("rise_sdf_amd ops only accept device (HIP) tensors; there is no CPU path")
     lead = x.shape[:-1]
-    n = x.numel() // x.shape[-1]
+    n = x.numel() // d
     if n == 0:                        # no rows: an empty, or zero, loss that still reaches its inputs' graph
         zero = x.sum().float() * 0.0 + weight.reshape(-1)[:1].sum().float() * 0.0
         return zero.expand(0).reshape(lead) if reduction == "none" else torch.nan_to_num(zero)
     k = 1 if logits is None else ids.shape[-1]
-    out = _ClassHead.apply(x.reshape(n, x.shape[-1]), weight, ids.reshape(n, k),
-                           None if logits is None else _f(logits).reshape(n, k), int(ignore), float(temperature),
+    out = _ClassHead.apply(x if x.dim() == 2 else x.reshape(n, d), weight, ids, logits, k, int(ignore), float(temperature),
                            _REDUCTIONS[reduction])
-    return out.reshape(lead) if reduction == "none" else out
+    return out.reshape(lead) if reduction == "none" and len(lead) != 1 else out
 
 
 def linear_cross_entropy(x, weight, target, *, ignore_index=-100, reduction="mean"):
@@ -219,7 +226,7 @@ def linear_cross_entropy(x, weight, target, *, ignore_index=-100, reduction="mea
     Differentiable w.r.t. ``x`` and ``weight`` (once).  Rows with ``target == ignore_index`` take part in nothing, whatever
     ``x`` holds there; any other target outside [0, V) makes its row NaN, takes no part in the gradients and is reported by
     ``rise_sdf_amd.check_status()``."""
-    if tuple(target.shape) != tuple(x.shape[:-1]):
+    if target.shape != x.shape[:-1]:
         raise L.RiseSdfHipError(f"linear_cross_entropy: one target per row: {tuple(target.shape)} for features "
                                 f"{tuple(x.shape)}")
     return _class_head("linear_cross_entropy", x, weight, target, None, ignore_index, 1.0, reduction)

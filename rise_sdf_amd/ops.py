@@ -711,46 +711,55 @@ def _dtype_id(t, what):
 
 def _same_device(what, *tensors):
     dev = tensors[0].device
-    if any(t.device != dev for t in tensors):
-        raise L.RiseSdfHipError(f"{what}: tensors on different devices ({', '.join(str(t.device) for t in tensors)})")
+    for t in tensors:
+        if t.device != dev:
+            raise L.RiseSdfHipError(f"{what}: tensors on different devices ({', '.join(str(t.device) for t in tensors)})")
     return dev
 
 
 def _int_ids(ids, what):
+    if ids.dtype is torch.int64 and ids.is_contiguous():
+        return ids
     if ids.dtype not in (torch.int64, torch.int32, torch.int16, torch.uint8):
         raise L.RiseSdfHipError(f"{what}: integer ids, not {ids.dtype}")
-    return ids.detach().to(torch.int64).contiguous()
+    return ids.to(torch.int64).contiguous()
+
+
+def once(backward):
+    """Backward of a Function that cannot be differentiated again: ``once_differentiable`` where a second derivative could be
+    asked for (create_graph), and without its cost where it cannot."""
+    guarded = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
 
 
 class _Embedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ids, table, scale, padding):
-        tb = table.detach().contiguous()
-        dt = _dtype_id(tb, "embedding")
-        require_device(ids, tb)
-        dev = _same_device("embedding", ids, tb)
+        tb = table if table.is_contiguous() else table.contiguous()
         V, D = tb.shape
-        with torch.cuda.device(dev):
-            out = torch.empty(*ids.shape, D, dtype=tb.dtype, device=dev)
-            check(lib().rsdf_embedding_fwd(ptr(ids), ids.numel(), ptr(tb), V, D, dt, scale, padding, ptr(out),
-                                           L.bad_ids_ptr(dev), stream_ptr()), "embedding_fwd")
+        dev = tb.get_device()
+        out = torch.empty(*ids.shape, D, dtype=tb.dtype, device=tb.device)
+        L.launch(dev, lib().rsdf_embedding_fwd, "embedding_fwd", ids.data_ptr(), ids.numel(), tb.data_ptr(), V, D,
+                 DTYPE_IDS[tb.dtype], scale, padding, out.data_ptr(), L.bad_ids_ptr(dev))
         ctx.save_for_backward(ids)
-        ctx.shape, ctx.dtype, ctx.scale, ctx.padding = (V, D), tb.dtype, scale, padding
+        ctx.state = V, D, tb.dtype, scale, padding
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once
     def backward(ctx, gout):
         (ids,) = ctx.saved_tensors
-        V, D = ctx.shape
-        g = gout.detach().to(ctx.dtype).contiguous()
-        n, dev = ids.numel(), ids.device
-        with torch.cuda.device(dev):
-            dt = torch.empty(V, D, dtype=ctx.dtype, device=dev)
-            nbytes = int(lib().rsdf_embedding_bwd_workspace_bytes(n, V, D))
-            ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
-            check(lib().rsdf_embedding_bwd(ptr(ids), n, ptr(g), V, D, DTYPE_IDS[ctx.dtype], ctx.scale, ctx.padding, ptr(dt),
-                                           ptr(ws), nbytes, stream_ptr()), "embedding_bwd")
+        V, D, dtype, scale, padding = ctx.state
+        g = gout if gout.dtype is dtype and gout.is_contiguous() else gout.to(dtype).contiguous()
+        n, l = ids.numel(), lib()
+        dt = torch.empty(V, D, dtype=dtype, device=ids.device)
+        nbytes = l.rsdf_embedding_bwd_workspace_bytes(n, V, D)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=ids.device) if nbytes > 0 else None
+        L.launch(ids.get_device(), l.rsdf_embedding_bwd, "embedding_bwd", ids.data_ptr(), n, g.data_ptr(), V, D, DTYPE_IDS[dtype],
+                 scale, padding, dt.data_ptr(), None if ws is None else ws.data_ptr(), nbytes)
         return None, dt, None, None
 
 
@@ -764,12 +773,16 @@ def embedding(ids, table, scale=1.0, padding_idx=None):
     if not torch.is_tensor(table) or table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1:
         raise L.RiseSdfHipError("embedding: table must be [V, D] with V, D >= 1")
     _dtype_id(table, "embedding")
+    ids = _int_ids(ids, "embedding")
     pad = _NO_PADDING
     if padding_idx is not None:
         pad = int(padding_idx)
         if not 0 <= pad < table.shape[0]:
             raise L.RiseSdfHipError(f"embedding: padding_idx {pad} outside the table's {table.shape[0]} rows")
-    return _Embedding.apply(_int_ids(ids, "embedding"), table, float(scale), pad)
+    if not (table.is_cuda and ids.is_cuda):
+        raise L.RiseSdfHipError("rise_sdf_amd ops only accept device (HIP) tensors; there is no CPU path")
+    _same_device("embedding", ids, table)
+    return _Embedding.apply(ids, table, float(scale), pad)
 
 
 # ------------------------------------------------------------------------------------------------
