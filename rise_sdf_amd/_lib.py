@@ -328,14 +328,27 @@ def stream_ptr():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
-def launch(device_index, fn, what, *args):
-    """``fn(*args, stream)`` on the current stream of device ``device_index`` (which need not be the current device), checked.
-    Pointers are plain integers here: the caller's tensors stay alive in its own variables until the call has returned."""
-    if torch._C._cuda_getDevice() == device_index:
-        check(fn(*args, torch._C._cuda_getCurrentRawStream(device_index)), what)
-    else:
-        with torch.cuda.device(device_index):
-            check(fn(*args, torch._C._cuda_getCurrentRawStream(device_index)), what)
+NODES_PATH = os.path.join(_HERE, "_codebook.so")
+_nodes = None
+
+
+def nodes():
+    """The C++ autograd nodes of the codebook operators (csrc/codebook_torch.cpp), bound to the loaded library."""
+    global _nodes
+    if _nodes is None:
+        import importlib.util
+        lib()
+        if not os.path.exists(NODES_PATH):
+            raise RiseSdfHipError(f"{NODES_PATH} is missing: build it first (python -c 'import __graft_entry__ as g; g.build()' or "
+                                  "make -C rise_sdf_amd/csrc)")
+        spec = importlib.util.spec_from_file_location("_codebook", NODES_PATH)
+        m = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(m)
+        m.bind([ctypes.cast(getattr(_lib, "rsdf_" + n), ctypes.c_void_p).value for n in
+                ("last_error", "embedding_fwd", "embedding_bwd_workspace_bytes", "embedding_bwd", "class_head_workspace_bytes",
+                 "class_head_fwd", "class_head_bwd")], RiseSdfHipError)
+        _nodes = m
+    return _nodes
 
 
 # ---- transient workspaces -----------------------------------------------------------------------------------------------
@@ -482,12 +495,12 @@ _BAD_IDS_PTR = {}
 
 
 def bad_ids_ptr(idx):
-    """Address where kernels on device ``idx`` count ids outside their table (status word ST_BAD_IDS).  None while a graph is being
+    """Address where kernels on device ``idx`` count ids outside their table (status word ST_BAD_IDS).  0 (do not count) while a graph is being
     captured on a device that has no status words yet: they would live in the graph's private pool."""
     p = _BAD_IDS_PTR.get(idx)
     if p is None:
         if idx not in _STATUS and torch.cuda.is_current_stream_capturing():
-            return None
+            return 0
         p = _BAD_IDS_PTR[idx] = status(torch.device("cuda", idx)).data_ptr() + 4 * ST_BAD_IDS
     return p
 

@@ -1,0 +1,206 @@
+// Autograd nodes of the codebook operators (ops.embedding, loss.linear_cross_entropy, loss.linear_distillation) in C++: what
+// their small calls cost is the host's time, and a node in Python cost as much in the backward thread as all the launches of
+// the pass (lookup of 256 x 48 with its gradient: 71 us a call that way, of which 6 on the GPU).  The entry points of
+// librisesdf_hip.so come in as addresses (bind), so that this module works with whichever build of the library is loaded.
+// Host code only: no kernels here.
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/extension.h>
+
+namespace {
+
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+struct Error : std::runtime_error { using std::runtime_error::runtime_error; };
+
+struct Entries {
+    const char *(*last_error)();
+    int (*embedding_fwd)(const int64_t *, int64_t, const void *, int64_t, int, int, float, int64_t, void *, int32_t *, void *);
+    int64_t (*embedding_bwd_workspace_bytes)(int64_t, int64_t, int);
+    int (*embedding_bwd)(const int64_t *, int64_t, const void *, int64_t, int, int, float, int64_t, void *, void *, int64_t, void *);
+    int64_t (*class_head_workspace_bytes)(int64_t, int64_t, int, int, int);
+    int (*class_head_fwd)(const void *, const void *, int64_t, int64_t, int, int, const int64_t *, const float *, int, int64_t, float, int,
+                          float *, float *, float *, float *, float *, int32_t *, void *, int64_t, void *);
+    int (*class_head_bwd)(const void *, const void *, int64_t, int64_t, int, int, const int64_t *, const float *, const float *, int, float,
+                          const float *, const float *, const float *, int, void *, void *, void *, int64_t, void *);
+} E = {};
+
+void *stream_of(const Tensor &t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
+
+void check(int rc, const char *what)
+{
+    if (rc == 0) return;
+    const char *msg = E.last_error();
+    throw Error(std::string(what) + " failed (code " + std::to_string(rc) + "): " + (msg != nullptr ? msg : ""));
+}
+
+int dtype_id(const Tensor &t)
+{
+    return t.scalar_type() == at::kFloat ? 0 : (t.scalar_type() == at::kBFloat16 ? 1 : 2);       // (the caller checked)
+}
+
+Tensor bytes_on(int64_t n, const Tensor &like)
+{
+    return at::empty({n}, like.options().dtype(at::kByte).requires_grad(false));
+}
+
+template <class T> T *address(const Tensor &t) { return t.defined() ? (T *)t.data_ptr() : nullptr; }
+
+// gradients of a node that cannot be differentiated again: under create_graph a second derivative raises instead of being zero
+variable_list once(variable_list grads, const char *what)
+{
+    if (!at::GradMode::is_enabled()) return grads;
+    variable_list there;
+    for (auto &g : grads)
+        if (g.defined()) there.push_back(g.detach().requires_grad_(true));
+    if (there.empty()) return grads;
+    auto error = std::make_shared<torch::autograd::DelayedError>(std::string(what) + " cannot be differentiated twice", (int)there.size());
+    auto out = (*error)(std::move(there));
+    size_t i = 0;
+    for (auto &g : grads)
+        if (g.defined()) g = out[i++];
+    return grads;
+}
+
+struct Embedding : torch::autograd::Function<Embedding> {
+    static Tensor forward(AutogradContext *ctx, const Tensor &ids, const Tensor &table_, double scale, int64_t padding, int64_t bad_ids)
+    {
+        const Tensor table = table_.contiguous();
+        const c10::DeviceGuard guard(table.device());
+        const int64_t v = table.size(0), d = table.size(1);
+        auto shape = ids.sizes().vec();
+        shape.push_back(d);
+        Tensor out = at::empty(shape, table.options().requires_grad(false));
+        check(E.embedding_fwd(address<const int64_t>(ids), ids.numel(), address<const void>(table), v, (int)d, dtype_id(table), (float)scale,
+                              padding, address<void>(out), (int32_t *)bad_ids, stream_of(table)),
+              "embedding_fwd");
+        ctx->save_for_backward({ids});
+        ctx->saved_data["v"] = v;
+        ctx->saved_data["d"] = d;
+        ctx->saved_data["type"] = (int64_t)table.scalar_type();
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["padding"] = padding;
+        return out;
+    }
+
+    static variable_list backward(AutogradContext *ctx, variable_list grads)
+    {
+        const Tensor ids = ctx->get_saved_variables()[0];
+        const int64_t v = ctx->saved_data["v"].toInt(), d = ctx->saved_data["d"].toInt(), n = ids.numel();
+        const c10::DeviceGuard guard(ids.device());
+        const Tensor g = grads[0].detach().to((at::ScalarType)ctx->saved_data["type"].toInt()).contiguous();
+        Tensor dt = at::empty({v, d}, g.options());
+        const int64_t bytes = E.embedding_bwd_workspace_bytes(n, v, (int)d);
+        const Tensor ws = bytes > 0 ? bytes_on(bytes, g) : Tensor();
+        check(E.embedding_bwd(address<const int64_t>(ids), n, address<const void>(g), v, (int)d, dtype_id(g),
+                              (float)ctx->saved_data["scale"].toDouble(), ctx->saved_data["padding"].toInt(), address<void>(dt),
+                              address<void>(ws), bytes, stream_of(g)),
+              "embedding_bwd");
+        return once({Tensor(), dt, Tensor(), Tensor(), Tensor()}, "embedding");
+    }
+};
+
+// contiguous and 16-byte aligned (a view into the middle of a storage may be neither)
+Tensor aligned(const Tensor &t)
+{
+    const Tensor c = t.detach().contiguous();
+    return ((uintptr_t)c.data_ptr() & 15) == 0 ? c : c.clone();
+}
+
+// both losses: no logits = labels (k = 1), else a teacher's listed classes
+struct ClassHead : torch::autograd::Function<ClassHead> {
+    static Tensor forward(AutogradContext *ctx, const Tensor &x_, const Tensor &w_, const Tensor &ids, const c10::optional<Tensor> &logits,
+                          int64_t k, int64_t ignore, double temperature, int64_t reduction, int64_t bad_ids)
+    {
+        const Tensor x = aligned(x_), w = aligned(w_);
+        const c10::DeviceGuard guard(x.device());
+        const int64_t n = x.size(0), d = x.size(1), v = w.size(0);
+        const bool teacher = logits.has_value();
+        const int64_t bytes = E.class_head_workspace_bytes(n, v, (int)d, dtype_id(x), 0);
+        if (bytes < 0) check(1, "class_head_workspace_bytes");
+        const Tensor ws = bytes_on(bytes, x);
+        const auto f32 = x.options().dtype(at::kFloat).requires_grad(false);
+        // lse [n], count [1], and for a teacher q, listed logits [n, k]: one allocation, kept for the backward
+        const Tensor keep = at::empty({n + 1 + (teacher ? 2 * n * k : 0)}, f32);
+        Tensor loss = reduction == 0 ? at::empty({n}, f32) : at::empty({}, f32);
+        float *a = address<float>(keep), *q = teacher ? a + n + 1 : nullptr;
+        check(E.class_head_fwd(address<const void>(x), address<const void>(w), n, v, (int)d, dtype_id(x), address<const int64_t>(ids),
+                               teacher ? address<const float>(*logits) : nullptr, (int)k, ignore, (float)temperature, (int)reduction,
+                               address<float>(loss), a, a + n, q, teacher ? q + n * k : nullptr, (int32_t *)bad_ids, address<void>(ws), bytes,
+                               stream_of(x)),
+              "class_head_fwd");
+        ctx->save_for_backward({x, w, ids, keep});
+        ctx->saved_data["k"] = k;
+        ctx->saved_data["temperature"] = temperature;
+        ctx->saved_data["reduction"] = reduction;
+        ctx->saved_data["teacher"] = teacher;
+        return loss;
+    }
+
+    static variable_list backward(AutogradContext *ctx, variable_list grads)
+    {
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &x = saved[0], &w = saved[1], &ids = saved[2], &keep = saved[3];
+        const int64_t n = x.size(0), d = x.size(1), v = w.size(0), k = ctx->saved_data["k"].toInt();
+        const int64_t reduction = ctx->saved_data["reduction"].toInt();
+        const bool teacher = ctx->saved_data["teacher"].toBool();
+        const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
+        variable_list out(9);
+        if (!need_x && !need_w) return out;
+        const c10::DeviceGuard guard(x.device());
+        const Tensor g = grads[0].detach().to(at::kFloat).contiguous();
+        if (need_x) out[0] = at::empty_like(x);
+        if (need_w) out[1] = at::empty_like(w);
+        const int64_t bytes = E.class_head_workspace_bytes(n, v, (int)d, dtype_id(x), (need_x ? 1 : 0) + (need_w ? 2 : 0));
+        const Tensor ws = bytes_on(bytes, x);
+        float *a = address<float>(keep), *q = teacher ? a + n + 1 : nullptr;
+        check(E.class_head_bwd(address<const void>(x), address<const void>(w), n, v, (int)d, dtype_id(x), address<const int64_t>(ids), q,
+                               teacher ? q + n * k : nullptr, (int)k, (float)ctx->saved_data["temperature"].toDouble(), a,
+                               reduction == 1 ? a + n : nullptr, address<const float>(g), reduction == 0, address<void>(out[0]),
+                               address<void>(out[1]), address<void>(ws), bytes, stream_of(x)),
+              "class_head_bwd");
+        return once(std::move(out), "the losses of a linear head");
+    }
+};
+
+void bind(const std::vector<uintptr_t> &a, py::object error)
+{
+    TORCH_CHECK(a.size() == 7, "seven entry points");
+    static py::object *type = nullptr;       // (kept for the life of the process)
+    if (type != nullptr) return;
+    type = new py::object(error);
+    py::register_exception_translator([](std::exception_ptr p) {
+        try {
+            if (p) std::rethrow_exception(p);
+        } catch (const Error &e) {
+            PyErr_SetString(type->ptr(), e.what());
+        }
+    });
+    E.last_error = (decltype(E.last_error))a[0];
+    E.embedding_fwd = (decltype(E.embedding_fwd))a[1];
+    E.embedding_bwd_workspace_bytes = (decltype(E.embedding_bwd_workspace_bytes))a[2];
+    E.embedding_bwd = (decltype(E.embedding_bwd))a[3];
+    E.class_head_workspace_bytes = (decltype(E.class_head_workspace_bytes))a[4];
+    E.class_head_fwd = (decltype(E.class_head_fwd))a[5];
+    E.class_head_bwd = (decltype(E.class_head_bwd))a[6];
+}
+
+}  // namespace
+
+PYBIND11_MODULE(_codebook, m)
+{
+    m.def("bind", &bind);
+    m.def("embedding", [](const Tensor &ids, const Tensor &table, double scale, int64_t padding, int64_t bad_ids) {
+        py::gil_scoped_release free;
+        return Embedding::apply(ids, table, scale, padding, bad_ids);
+    });
+    m.def("class_head", [](const Tensor &x, const Tensor &w, const Tensor &ids, const c10::optional<Tensor> &logits, int64_t k, int64_t ignore,
+                           double temperature, int64_t reduction, int64_t bad_ids) {
+        py::gil_scoped_release free;
+        return ClassHead::apply(x, w, ids, logits, k, ignore, temperature, reduction, bad_ids);
+    });
+}

@@ -14,7 +14,7 @@ import torch
 
 from . import _lib as L
 from ._lib import check, lib, ptr, require_device, stream_ptr
-from .ops import DTYPE_IDS, _dtype_id, _int_ids, _same_device, once
+from .ops import _dtype_id, _int_ids, _same_device
 
 
 def _f(t):
@@ -127,65 +127,6 @@ def loss_tail(out, batch, lambdas, sparsity_scale=1.0, has_mask=True):
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 
 
-def _aligned(t):
-    """Contiguous and 16-byte aligned (a view into the middle of a storage may be neither)."""
-    if not t.is_contiguous():
-        return t.detach().contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.detach().clone()
-
-
-def _addr(t):
-    return None if t is None else t.data_ptr()
-
-
-class _ClassHead(torch.autograd.Function):
-    """Both losses: ``logits`` None = labels (``ids`` [N, 1]), else a teacher's listed classes (``ids``, ``logits`` [N, K])."""
-
-    @staticmethod
-    def forward(ctx, x, w, ids, logits, k, ignore, temperature, reduction):
-        xc, wc = _aligned(x), _aligned(w)
-        (n, d), v, device, l = xc.shape, wc.shape[0], xc.device, lib()
-        dt = DTYPE_IDS[xc.dtype]
-        nbytes = l.rsdf_class_head_workspace_bytes(n, v, d, dt, 0)
-        if nbytes < 0:
-            check(1, "class_head_workspace_bytes")
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        # lse [n], count [1], and for a teacher q, listed logits [n, k]: one allocation, kept for the backward
-        keep = torch.empty(n + 1 + (2 * n * k if logits is not None else 0), dtype=torch.float32, device=device)
-        loss = torch.empty(n if reduction == 0 else (), dtype=torch.float32, device=device)
-        a = keep.data_ptr()
-        q, zt = (a + 4 * (n + 1), a + 4 * (n + 1 + n * k)) if logits is not None else (None, None)
-        dev = xc.get_device()
-        L.launch(dev, l.rsdf_class_head_fwd, "class_head_fwd", xc.data_ptr(), wc.data_ptr(), n, v, d, dt, ids.data_ptr(),
-                 _addr(logits), k, ignore, temperature, reduction, loss.data_ptr(), a, a + 4 * n, q, zt, L.bad_ids_ptr(dev),
-                 ws.data_ptr(), nbytes)
-        ctx.save_for_backward(xc, wc, ids, keep)
-        ctx.state = k, temperature, reduction, logits is not None
-        return loss
-
-    @staticmethod
-    @once
-    def backward(ctx, g):
-        xc, wc, ids, keep = ctx.saved_tensors
-        k, temperature, reduction, teacher = ctx.state
-        need_x, need_w = ctx.needs_input_grad[:2]
-        if not (need_x or need_w):
-            return (None,) * 8
-        (n, d), v, l = xc.shape, wc.shape[0], lib()
-        dt = DTYPE_IDS[xc.dtype]
-        g = g if g.is_contiguous() else g.contiguous()
-        dx = torch.empty_like(xc) if need_x else None
-        dw = torch.empty_like(wc) if need_w else None
-        nbytes = l.rsdf_class_head_workspace_bytes(n, v, d, dt, int(need_x) + 2 * int(need_w))
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=xc.device)
-        a = keep.data_ptr()
-        q, zt = (a + 4 * (n + 1), a + 4 * (n + 1 + n * k)) if teacher else (None, None)
-        L.launch(xc.get_device(), l.rsdf_class_head_bwd, "class_head_bwd", xc.data_ptr(), wc.data_ptr(), n, v, d, dt,
-                 ids.data_ptr(), q, zt, k, temperature, a, a + 4 * n if reduction == 1 else None, g.data_ptr(),
-                 int(reduction == 0), _addr(dx), _addr(dw), ws.data_ptr(), nbytes)
-        return dx, dw, None, None, None, None, None, None
-
-
 def _class_head(what, x, weight, ids, logits, ignore, temperature, reduction):
     err = L.RiseSdfHipError
     if reduction not in _REDUCTIONS:
@@ -212,8 +153,8 @@ def _class_head(what, x, weight, ids, logits, ignore, temperature, reduction):
         zero = x.sum().float() * 0.0 + weight.reshape(-1)[:1].sum().float() * 0.0
         return zero.expand(0).reshape(lead) if reduction == "none" else torch.nan_to_num(zero)
     k = 1 if logits is None else ids.shape[-1]
-    out = _ClassHead.apply(x if x.dim() == 2 else x.reshape(n, d), weight, ids, logits, k, int(ignore), float(temperature),
-                           _REDUCTIONS[reduction])
+    out = L.nodes().class_head(x if x.dim() == 2 else x.reshape(n, d), weight, ids, logits, k, int(ignore), float(temperature),
+                               _REDUCTIONS[reduction], L.bad_ids_ptr(x.get_device()))
     return out.reshape(lead) if reduction == "none" and len(lead) != 1 else out
 
 

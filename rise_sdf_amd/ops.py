@@ -725,44 +725,6 @@ def _int_ids(ids, what):
     return ids.to(torch.int64).contiguous()
 
 
-def once(backward):
-    """Backward of a Function that cannot be differentiated again: ``once_differentiable`` where a second derivative could be
-    asked for (create_graph), and without its cost where it cannot."""
-    guarded = torch.autograd.function.once_differentiable(backward)
-
-    def run(ctx, *grads):
-        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
-    return run
-
-
-class _Embedding(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, ids, table, scale, padding):
-        tb = table if table.is_contiguous() else table.contiguous()
-        V, D = tb.shape
-        dev = tb.get_device()
-        out = torch.empty(*ids.shape, D, dtype=tb.dtype, device=tb.device)
-        L.launch(dev, lib().rsdf_embedding_fwd, "embedding_fwd", ids.data_ptr(), ids.numel(), tb.data_ptr(), V, D,
-                 DTYPE_IDS[tb.dtype], scale, padding, out.data_ptr(), L.bad_ids_ptr(dev))
-        ctx.save_for_backward(ids)
-        ctx.state = V, D, tb.dtype, scale, padding
-        return out
-
-    @staticmethod
-    @once
-    def backward(ctx, gout):
-        (ids,) = ctx.saved_tensors
-        V, D, dtype, scale, padding = ctx.state
-        g = gout if gout.dtype is dtype and gout.is_contiguous() else gout.to(dtype).contiguous()
-        n, l = ids.numel(), lib()
-        dt = torch.empty(V, D, dtype=dtype, device=ids.device)
-        nbytes = l.rsdf_embedding_bwd_workspace_bytes(n, V, D)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=ids.device) if nbytes > 0 else None
-        L.launch(ids.get_device(), l.rsdf_embedding_bwd, "embedding_bwd", ids.data_ptr(), n, g.data_ptr(), V, D, DTYPE_IDS[dtype],
-                 scale, padding, dt.data_ptr(), None if ws is None else ws.data_ptr(), nbytes)
-        return None, dt, None, None
-
-
 def embedding(ids, table, scale=1.0, padding_idx=None):
     """Codes by id: ``ids`` (integers, any shape) -> [*ids.shape, D] = ``scale * table[ids]`` for ``table`` [V, D] in fp32, bf16
     or fp16 (fp32 products, one rounding).  ``padding_idx``: the id whose rows are zero and take no gradient.
@@ -782,7 +744,7 @@ def embedding(ids, table, scale=1.0, padding_idx=None):
     if not (table.is_cuda and ids.is_cuda):
         raise L.RiseSdfHipError("rise_sdf_amd ops only accept device (HIP) tensors; there is no CPU path")
     _same_device("embedding", ids, table)
-    return _Embedding.apply(ids, table, float(scale), pad)
+    return L.nodes().embedding(ids, table, float(scale), pad, L.bad_ids_ptr(table.get_device()))
 
 
 # ------------------------------------------------------------------------------------------------

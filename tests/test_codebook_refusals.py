@@ -96,3 +96,18 @@ def test_embedding_encoding_on_the_cpu():
     assert list(e.state_dict()) == ["params"]
     with pytest.raises(NotImplementedError, match="Embedding"):
         get_encoding(3, Config({"otype": "Embedding", "n_embeddings": 7, "n_features": 5}))
+
+
+def test_missing_nodes_fail_loudly(tmp_path, monkeypatch):
+    monkeypatch.setattr(_lib, "_nodes", None)
+    monkeypatch.setattr(_lib, "NODES_PATH", str(tmp_path / "nope.so"))
+    with pytest.raises(ERR, match="missing"):
+        _lib.nodes()
+
+
+def test_nodes_load_and_report_errors_as_the_library_does():
+    """Without a device: the nodes bind to the loaded library, and a refused size comes back as the framework's error."""
+    n = _lib.nodes()
+    ids, table = torch.zeros(2, dtype=torch.int64), torch.zeros(3, (1 << 16) + 1)
+    with pytest.raises((ERR, RuntimeError)):
+        n.embedding(ids, table, 1.0, -1, 0)

@@ -484,3 +484,23 @@ def test_codes_through_a_network_into_both_losses(dev):
     for m, (w, b) in zip([m for m in field.network.layers if isinstance(m, torch.nn.Linear)], wb):
         close(m.weight.grad, w.grad)
         close(m.bias.grad, b.grad)
+
+
+def test_second_derivatives_are_refused(dev):
+    ids, table, _ = lookup_case(dev, 20, 10, 4, F32)
+    x, w, y = head_case(dev, 20, 30, 8, F32)
+    for out, leaf in ((ops.embedding(ids, table.requires_grad_(True)).square().sum(), table),
+                      (linear_cross_entropy(x.requires_grad_(True), w, y), x)):
+        (g,) = torch.autograd.grad(out, leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiated twice"):
+            g.square().sum().backward()
+
+
+def test_saved_tensors_changed_in_place_are_noticed(dev):
+    x, w, y = head_case(dev, 20, 30, 8, F32)
+    w.requires_grad_(True)
+    loss = linear_cross_entropy(x, w, y)
+    with torch.no_grad():
+        w.mul_(2.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
