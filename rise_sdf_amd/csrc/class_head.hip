@@ -208,16 +208,29 @@ struct RowState {
     int label[TL::NT];
     __device__ __forceinline__ void load(const HeadArgs &a, int64_t m0, int64_t n0)
     {
-        const float top = a.top[0];
+        const int rows = (int)(a.n - n0 < TL::BN ? a.n - n0 : TL::BN);
+        const float *pl = a.lse + n0, *pw = a.weight + n0;
+        const int *pt = a.label != nullptr ? (const int *)(a.label + n0) : (const int *)pl;
+        const int two = a.label != nullptr ? 2 : 1;
 #pragma unroll
         for (int nt = 0; nt < TL::NT; ++nt) {
-            const int64_t n = n0 + TL::n_of(nt);
-            lse[nt] = n < a.n ? a.lse[n] : __builtin_inff();
-            f[nt] = lse[nt] != __builtin_inff() ? a.weight[n] / top * (TL::F16 ? F16_DZ : 1.0f) : 0.0f;
-            const int64_t l = (f[nt] != 0.0f && a.label != nullptr) ? a.label[n] - a.v0 - m0 : -1;
-            label[nt] = l >= 0 && l < TL::BM ? (int)l : -1;
-            // here, and not behind the requests of the next tile: the loads' wait would wait for those too
-            asm volatile("" ::"v"(lse[nt]), "v"(f[nt]), "v"(label[nt]));
+            int n = TL::n_of(nt);
+            n = n < rows ? n : (rows > 0 ? rows - 1 : 0);
+            lse[nt] = rows > 0 ? pl[n] : __builtin_inff();
+            f[nt] = rows > 0 ? pw[n] : 0.0f;
+            label[nt] = rows > 0 ? pt[n * two] : 0;      // (the low half: a row that takes part has a label of this head)
+        }
+        const float top = a.top[0];
+        // here, and not behind the requests of the next tile: the loads' wait would wait for those too
+#pragma unroll
+        for (int nt = 0; nt < TL::NT; ++nt) asm volatile("" ::"v"(lse[nt]), "v"(f[nt]), "v"(label[nt]));
+        const int first = (int)(a.v0 + m0);
+#pragma unroll
+        for (int nt = 0; nt < TL::NT; ++nt) {
+            const bool live = TL::n_of(nt) < rows && lse[nt] != __builtin_inff();
+            lse[nt] = live ? lse[nt] : __builtin_inff();
+            f[nt] = live ? f[nt] / top * (TL::F16 ? F16_DZ : 1.0f) : 0.0f;      // (equal weights: exactly 1)
+            label[nt] = f[nt] != 0.0f && a.label != nullptr ? label[nt] - first : -1;
         }
     }
 };
@@ -229,7 +242,7 @@ __device__ __forceinline__ void head_results(const HeadArgs &a, typename TL::Acc
     const bool whole = a.vc - m0 >= TL::BM;     // else the last classes of the tile are not there
     const int left = whole ? TL::BM : (int)(a.vc - m0);      // (0 or less: a tile of zeros)
     if (!DZ) {
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / TL::WN;
+        const int lane = my_lane(), wm = my_wave() / TL::WN;
         if (!whole) {
 #pragma unroll
             for (int mt = 0; mt < TL::MT; ++mt) {
@@ -363,10 +376,13 @@ __global__ void __launch_bounds__(TL::THREADS, TL::OCCUPANCY) head_walk_kernel(H
     typename TL::Pipe pipe;
     head_tile<TL>(a, t, W, X, m0, n0);
     pipe.begin(W, X, a.nseg, ksteps, 0, steps, lds);
-    for (;;) {
+    // stores of dz by a wave behind the requests of its next tile (head_results: two per part, block of 64 classes and 16 rows)
+    constexpr int STORES = DZ ? 2 * PARTS * (TL::MT / 4) * TL::NT : 0;
+    static_assert(TL::LOW + TL::HIGH + STORES < 64, "vmcnt has six bits");
+    for (bool later = false;; later = true) {
         typename TL::Acc acc;
         clear<TL>(acc);
-        pipe.finish(acc);
+        pipe.template finish<STORES>(acc, later);
         RowState<TL> rows;
         if (DZ) rows.load(a, m0, n0);
         const int64_t m = m0, n = n0;

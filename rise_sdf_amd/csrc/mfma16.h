@@ -35,6 +35,10 @@ typedef const __attribute__((address_space(1))) void glob_void;
 
 constexpr int BK = 32;          // K of a matrix instruction
 
+// lane and wave of this thread; the lane is counted anew wherever it is needed instead of occupying a register in the main loop
+__device__ __forceinline__ int my_lane() { return (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u)); }
+__device__ __forceinline__ int my_wave() { return __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); }
+
 template <bool F16>
 __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c)
 {
@@ -114,7 +118,7 @@ struct Loader {
     __device__ __forceinline__ void next() { cur += COLS ? (int64_t)KD * row_bytes : KD * 2; }
 
     // request this step into the LDS image `dst`; k_left >= 1: valid k from here on
-    __device__ __forceinline__ void issue(unsigned char *dst, int k_left, int wave, int lane) const
+    __device__ __forceinline__ void issue(unsigned char *dst, int k_left, int wave) const
     {
         unsigned bo[PER_WAVE];
 #pragma unroll
@@ -122,7 +126,7 @@ struct Loader {
         if (COLS && k_left < KD) {
 #pragma unroll
             for (int j = 0; j < PER_WAVE; ++j) {
-                const int row = ((j * WAVES + wave) * 64 + lane) / CHUNKS;
+                const int row = ((j * WAVES + wave) * 64 + my_lane()) / CHUNKS;
                 if (row >= k_left) bo[j] -= (unsigned)(row - (k_left - 1)) * row_bytes;
             }
         }
@@ -203,7 +207,7 @@ struct Tile {
     __device__ static __forceinline__ void run(Acc &acc, const Operand &A, const Operand &Bo, int nseg, int64_t ksteps, int64_t s0,
                                                int64_t s1, unsigned char *lds)
     {
-        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const int lane = my_lane(), wave = my_wave();
         const int wm = wave / WN, wn = wave % WN;
         LA la;
         LB lb;
@@ -216,8 +220,8 @@ struct Tile {
         la.seek(A, seg_a(seg, nseg), kk);
         lb.seek(Bo, seg_b(seg, nseg), kk);
         auto request = [&]() {
-            la.issue(put, A.k_rows - kk * KD, wave, lane);
-            lb.issue(put + A_BYTES, Bo.k_rows - kk * KD, wave, lane);
+            la.issue(put, A.k_rows - kk * KD, wave);
+            lb.issue(put + A_BYTES, Bo.k_rows - kk * KD, wave);
             put = put == lds + (STAGES - 1) * STAGE ? lds : put + STAGE;
             la.next();
             lb.next();
@@ -261,20 +265,18 @@ struct Tile {
     // first m (inside the tile) of the 16 consecutive ones that acc[4 blk .. 4 blk + 3] hold, and the n of acc[.][nt]
     __device__ static __forceinline__ int m_of(int blk)
     {
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-        return (wave / WN) * TM + blk * 64 + (lane >> 4) * 16;
+        return (my_wave() / WN) * TM + blk * 64 + (my_lane() >> 4) * 16;
     }
     __device__ static __forceinline__ int n_of(int nt)
     {
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15;
-        const int base = (wave % WN) * TN;
+        const int i = my_lane() & 15, base = (my_wave() % WN) * TN;
         return BCOLS ? base + (nt >> 2) * 64 + (i >> 2) * 16 + (((nt & 3) ^ ((i >> 2) & 1)) << 2) + (i & 3) : base + nt * 16 + i;
     }
     // the four results at m_of(blk) + 4 j
     __device__ static __forceinline__ f32x4 quad(const Acc &acc, int blk, int j, int nt)
     {
         if (!ACOLS) return acc[4 * blk + j][nt];
-        const bool odd = (threadIdx.x >> 4) & 1;
+        const bool odd = (my_lane() >> 4) & 1;
         const f32x4 a = acc[4 * blk + j][nt], b = acc[4 * blk + (j ^ 1)][nt];
         return f32x4{odd ? b[0] : a[0], odd ? b[1] : a[1], odd ? b[2] : a[2], odd ? b[3] : a[3]};
     }
@@ -318,14 +320,14 @@ struct DuoTile : Tile<BM_, BN_, WM_, WN_, ACOLS_, BCOLS_, F16_> {
         LB lb;
         Operand A, B;
         int nseg, last_k, steps, seg_lo, k_lo, seg_hi, k_hi;
-        int lane, wave;
+        int wave;
         unsigned char *lds;
 
         // step s of n and the lower half of m; of the upper half: both are called for s = 0, 1, ...
         __device__ __forceinline__ void request_low(unsigned char *img)
         {
-            lb.issue(img + 2 * HALF, B.k_rows - k_lo * KD, wave, lane);
-            lo.issue(img, A.k_rows - k_lo * KD, wave, lane);
+            lb.issue(img + 2 * HALF, B.k_rows - k_lo * KD, wave);
+            lo.issue(img, A.k_rows - k_lo * KD, wave);
             lb.next();
             lo.next();
             if (++k_lo == last_k && ++seg_lo < nseg) {
@@ -336,7 +338,7 @@ struct DuoTile : Tile<BM_, BN_, WM_, WN_, ACOLS_, BCOLS_, F16_> {
         }
         __device__ __forceinline__ void request_high(unsigned char *img)
         {
-            hi.issue(img + HALF, A.k_rows - k_hi * KD, wave, lane);
+            hi.issue(img + HALF, A.k_rows - k_hi * KD, wave);
             hi.next();
             if (++k_hi == last_k && ++seg_hi < nseg) {
                 k_hi = 0;
@@ -349,8 +351,8 @@ struct DuoTile : Tile<BM_, BN_, WM_, WN_, ACOLS_, BCOLS_, F16_> {
                                               unsigned char *lds_)
         {
             A = A_; B = B_; nseg = nseg_; lds = lds_;
-            lane = threadIdx.x & 63;
-            wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+            wave = my_wave();
+            const int lane = my_lane();
             last_k = (int)ksteps;
             steps = (int)(s1 - s0);
             lo.init(A, wave, lane, 0);
@@ -368,9 +370,12 @@ struct DuoTile : Tile<BM_, BN_, WM_, WN_, ACOLS_, BCOLS_, F16_> {
             if (steps > 1) request_low(lds + STAGE);
         }
 
-        __device__ __forceinline__ void finish(Acc &acc)
+        // AFTER: requests to memory (stores) of this wave between begin() and here, if `after_begin`: the waits for what begin() asked
+        // for need not wait for them
+        template <int AFTER = 0>
+        __device__ __forceinline__ void finish(Acc &acc, bool after_begin = false)
         {
-            const int wm = wave / WN, wn = wave % WN;
+            const int lane = my_lane(), wm = wave / WN, wn = wave % WN;
             const bool second = wave >= 4;
             u32x4 a[2][4], b[2][NT];
             auto read_a = [&](const unsigned char *half) {
@@ -390,12 +395,16 @@ struct DuoTile : Tile<BM_, BN_, WM_, WN_, ACOLS_, BCOLS_, F16_> {
                 __builtin_amdgcn_s_setprio(0);
             };
             unsigned char *img = lds, *other = lds + STAGE;
-            if (steps > 1) arrived<LOW + HIGH>();
-            else arrived<0>();
+            auto in_but = [&](bool more, bool first) {           // all but the last LOW + HIGH requests (and the stores) are in
+                if (!more) arrived<0>();
+                else if (first) arrived<LOW + HIGH + AFTER>();
+                else arrived<LOW + HIGH>();
+            };
+            in_but(steps > 1, after_begin);
             swap();
             if (second) swap();                               // one phase behind
             for (int s = 0; s < steps; ++s) {
-                const bool next = s + 1 < steps, after = s + 2 < steps;
+                const bool next = s + 1 < steps, after = s + 2 < steps, first = after_begin && s == 0;
                 // upper m of the other image: step s - 1 was read there a phase ago by both groups
 #pragma unroll
                 for (int k = 0; k < 2; ++k)
@@ -405,29 +414,17 @@ struct DuoTile : Tile<BM_, BN_, WM_, WN_, ACOLS_, BCOLS_, F16_> {
                 if (next) request_high(other);
                 // what the first group reads in its next phase has to be in by the end of the phase before it: the first group's
                 // own products, the second group's reads
-                if (second) {
-                    if (next) arrived<LOW + HIGH>();
-                    else arrived<0>();
-                }
+                if (second) in_but(next, first);
                 swap();
                 multiply(0);
-                if (!second) {
-                    if (next) arrived<LOW + HIGH>();
-                    else arrived<0>();
-                }
+                if (!second) in_but(next, first);
                 swap();
                 read_a(img + HALF);
                 if (after) request_low(img);                  // n and lower m of this image: both groups have read them
-                if (second) {
-                    if (after) arrived<LOW + HIGH>();
-                    else arrived<0>();
-                }
+                if (second) in_but(after, first);
                 swap();
                 multiply(4);
-                if (!second) {
-                    if (after) arrived<LOW + HIGH>();
-                    else arrived<0>();
-                }
+                if (!second) in_but(after, first);
                 swap();
                 unsigned char *t = img;
                 img = other;
