@@ -32,8 +32,7 @@ constexpr int T_F32 = 0, T_BF16 = 1, T_F16 = 2;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float F16_DZ = 4096.0f;
 constexpr int64_t DZ_BYTES = 128ll << 20;      // of one piece of dz
-constexpr int MIN_JOB = 12;                     // steps of 64: 4 / 8 / 16 / 24 took 38.3 / 31.4 / 26.4 / 29.2 us of products and joining at
-                                                // 4096 x 1000 x 48 fp32, 44.8 / 41.1 / 38.7 / 45.1 at 1001 x 10007 x 200 fp16
+constexpr double JOB_STEPS = 6.0;                // of a job of the products beyond its own steps
 constexpr int CUS = 256;                        // MI355X
 constexpr int64_t WPACK_BYTES = 128ll << 20;   // of the packed class codes of one piece
 
@@ -708,18 +707,20 @@ __device__ __forceinline__ void product(const ProdArgs &a, int64_t job, unsigned
 // dw of a piece (TW) and its share of dx (TX) in one launch: together they fill the chip with workgroups of about the same number
 // of steps, and dz is read by both while it is still in the last-level cache
 template <class TW, class TX, int DT>
-__global__ void __launch_bounds__(TW::THREADS, TW::OCCUPANCY) products_kernel(ProdArgs w, ProdArgs x)
+__global__ void __launch_bounds__(TW::THREADS, TW::OCCUPANCY) products_kernel(ProdArgs w, ProdArgs x, int x_first)
 {
     static_assert(TW::LDS == TX::LDS && TW::THREADS == TX::THREADS, "one workgroup shape");
     __shared__ __attribute__((aligned(1024))) unsigned char lds[TW::LDS];
-    // each XCD: a contiguous eighth of either list
-    const int64_t xcd = blockIdx.x & 7, i = blockIdx.x >> 3;
+    // each XCD: a contiguous eighth of either list, the longer jobs first
+    const int64_t xcd = blockIdx.x & 7;
     const int64_t jobs_w = w.tiles * w.splits, jobs_x = x.tiles * x.splits, per_w = (jobs_w + 7) / 8, per_x = (jobs_x + 7) / 8;
-    if (i < per_w) {
-        if (xcd * per_w + i < jobs_w) product<TW, DT>(w, xcd * per_w + i, lds);
+    int64_t i = blockIdx.x >> 3;
+    const bool is_x = x_first ? i < per_x : i >= per_w;
+    if (x_first ? !is_x : is_x) i -= x_first ? per_x : per_w;
+    if (is_x) {
+        if (i < per_x && xcd * per_x + i < jobs_x) product<TX, DT>(x, xcd * per_x + i, lds);
     } else {
-        const int64_t j = i - per_w;
-        if (j < per_x && xcd * per_x + j < jobs_x) product<TX, DT>(x, xcd * per_x + j, lds);
+        if (i < per_w && xcd * per_w + i < jobs_w) product<TW, DT>(w, xcd * per_w + i, lds);
     }
 }
 
@@ -780,6 +781,7 @@ struct Plan {
     bool small;                      // few rows: tiles of 32 rows
     int bm;                          // width of the d side of the products' tiles
     int split_dx, split_dw;
+    bool x_first;                    // the jobs of dx are the longer ones
 };
 
 Plan make_plan(int64_t n, int64_t v, int d, int dtype)
@@ -805,23 +807,34 @@ Plan make_plan(int64_t n, int64_t v, int d, int dtype)
     const int64_t pieces = (v + most - 1) / most;
     p.vc = up((v + pieces - 1) / pieces, 256);
     p.bm = d > 128 ? 256 : (d > 64 ? 128 : 64);
-    // The products of a piece are cut over k into jobs of about the same number of steps (64 deep), so many that they
-    // fill the chip once (BM 256: one workgroup per CU, else two), none below MIN_JOB steps.
+    // The products of a piece are cut over k into jobs of about `job` steps (64 deep); the cut with the least estimated time is
+    // taken.  In steps: a job's own cost (its first requests, its results), what the partial sums cost to write and read again,
+    // and for more jobs than the chip holds at once (BM 256: one per CU, else two) their average plus half a long one.
     const int bn = p.bm == 128 ? 128 : 256;
     const int64_t tm = (p.dp + p.bm - 1) / p.bm, seg = p.parts == 3 ? 6 : 1;
     const int64_t tiles_w = tm * ((p.vc + bn - 1) / bn), tiles_x = tm * ((n + bn - 1) / bn);
     const int64_t steps_w = seg * (up(n, 64) / 64), steps_x = seg * (p.vc / 64);
     const int64_t slots = p.bm == 256 ? CUS : 2 * CUS;
-    int64_t job = (tiles_w * steps_w + tiles_x * steps_x + slots - 1) / slots;
-    job = job < MIN_JOB ? MIN_JOB : job;
-    auto splits = [&](int64_t steps) {
-        const int64_t s = (steps + job - 1) / job;
-        return (int)(s < 1 ? 1 : (s > 64 ? 64 : s));
-    };
-    for (;; ++job) {
-        p.split_dx = splits(steps_x);
-        p.split_dw = splits(steps_w);
-        if (tiles_w * p.split_dw + tiles_x * p.split_dx <= slots || (p.split_dw == 1 && p.split_dx == 1)) break;
+    double best = 0.0;
+    for (int64_t job = 4;; job += job / 4 + 1) {
+        auto cut = [&](int64_t steps) {
+            const int64_t s = (steps + job - 1) / job;
+            return s < 1 ? (int64_t)1 : (s > 64 ? (int64_t)64 : s);
+        };
+        const int64_t sw = cut(steps_w), sx = cut(steps_x);
+        const double lw = (double)((steps_w + sw - 1) / sw) + JOB_STEPS, lx = (double)((steps_x + sx - 1) / sx) + JOB_STEPS;
+        const double jobs = (double)(tiles_w * sw + tiles_x * sx), all = tiles_w * sw * lw + tiles_x * sx * lx;
+        const double longest = lw > lx ? lw : lx;
+        double t = jobs <= slots ? longest : all / slots + longest / 2;
+        t = t > longest ? t : longest;
+        t += 8.0 * p.dp * (double)(sx * n + (sw > 1 ? sw * p.vc : 0)) / (p.bm == 256 ? 6.4e6 : 3.2e6);
+        if (best == 0.0 || t < best) {
+            best = t;
+            p.split_dw = (int)sw;
+            p.split_dx = (int)sx;
+            p.x_first = lx > lw;
+        }
+        if (sw == 1 && sx == 1) break;
     }
     return p;
 }
@@ -917,9 +930,9 @@ void launch_products(const Plan &p, ProdArgs w, ProdArgs x, hipStream_t st)
     w.tiles = w.rows > 0 ? w.tiles_m * ((w.rows + TW::BN - 1) / TW::BN) : 0;
     x.tiles = x.rows > 0 ? x.tiles_m * ((x.rows + TX::BN - 1) / TX::BN) : 0;
     const unsigned g = (unsigned)(8 * ((w.tiles * w.splits + 7) / 8 + (x.tiles * x.splits + 7) / 8));
-    if (p.dtype == T_F32) products_kernel<TW, TX, T_F32><<<g, TW::THREADS, 0, st>>>(w, x);
-    else if (TW::F16) products_kernel<TW, TX, T_F16><<<g, TW::THREADS, 0, st>>>(w, x);
-    else products_kernel<TW, TX, T_BF16><<<g, TW::THREADS, 0, st>>>(w, x);
+    if (p.dtype == T_F32) products_kernel<TW, TX, T_F32><<<g, TW::THREADS, 0, st>>>(w, x, p.x_first);
+    else if (TW::F16) products_kernel<TW, TX, T_F16><<<g, TW::THREADS, 0, st>>>(w, x, p.x_first);
+    else products_kernel<TW, TX, T_BF16><<<g, TW::THREADS, 0, st>>>(w, x, p.x_first);
 }
 template <bool F16>
 void products_of(const Plan &p, const ProdArgs &w, const ProdArgs &x, hipStream_t st)
