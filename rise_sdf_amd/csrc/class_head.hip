@@ -96,7 +96,7 @@ struct Pack { const void *src; int64_t rows, rows_pad; unsigned short *dst; };
 struct PrepArgs {
     Pack p[2];
     int64_t chunks[2];           // 8-element chunks of the two
-    int d, dp, wide;
+    int d, dp, unit;             // unit: bytes, the largest power of two (at most 16) that divides a row
     // weight of a row in the gradient: T g_n (mean: / count), 0 where it takes part in nothing; top[0] = the largest |weight|
     const float *lse, *g, *count;
     int g_per_row;
@@ -137,10 +137,20 @@ __global__ void __launch_bounds__(PREP) prep_kernel(PrepArgs a)
         bool live = r < p.rows;
         if (live && !second && a.lse != nullptr) live = a.lse[r] != __builtin_inff() && a.g[a.g_per_row ? r : 0] != 0.0f;
         float x[8];
-        if (live && a.wide && c + 8 <= a.d) {        // (rows are whole 16-byte pieces)
-            const u32x4 *s = (const u32x4 *)((const unsigned char *)p.src + (r * a.d + c) * (DT == T_F32 ? 4 : 2));
-            u32x4 raw[2] = {s[0], s[0]};
-            if (DT == T_F32) raw[1] = s[1];
+        if (live && c + 8 <= a.d && (DT != T_F32 ? a.unit >= 4 : a.unit >= 8)) {        // (rows start at multiples of the unit)
+            const unsigned char *s = (const unsigned char *)p.src + (r * a.d + c) * (DT == T_F32 ? 4 : 2);
+            unsigned raw[8];
+            constexpr int WORDS = DT == T_F32 ? 8 : 4;
+            if (a.unit == 16) {
+#pragma unroll
+                for (int i = 0; i < WORDS; i += 4) *(u32x4 *)(raw + i) = *(const u32x4 *)(s + 4 * i);
+            } else if (a.unit == 8) {
+#pragma unroll
+                for (int i = 0; i < WORDS; i += 2) *(uint2 *)(raw + i) = *(const uint2 *)(s + 4 * i);
+            } else {
+#pragma unroll
+                for (int i = 0; i < WORDS; ++i) raw[i] = *(const unsigned *)(s + 4 * i);
+            }
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[e] = load1<DT>(raw, e);
         } else {
@@ -169,7 +179,7 @@ struct HeadArgs {
     Operand w, x;                // base of the piece's first class / of row 0
     int64_t n, vc;               // rows, classes of the piece
     int nseg;
-    int64_t depth;               // K: a multiple of 64
+    int64_t depth;               // K: a multiple of 64 (zeros behind the features)
     float c;                     // log2(e) / T
     int64_t tiles_n, tiles;
     // statistics
@@ -413,32 +423,28 @@ struct RowArgs {
 // G dot products of row x with G rows of w by one wave: lane l gets number (l >> 3) & 7 of them.  The eight sums are folded
 // together, so that they cost 10 exchanges instead of 48.
 constexpr int G = 8;
-template <int DT, bool VEC>
+template <int E> struct Words { using type = u32x4; };
+template <> struct Words<8> { using type = uint2; };
+template <> struct Words<4> { using type = unsigned; };
+template <> struct Words<2> { using type = unsigned short; };
+template <int DT, int BYTES>
 __device__ __forceinline__ float dots(const void *x, const void *w, int64_t xo, const int64_t (&wo)[G], int d)
 {
-    constexpr int E = VEC ? (DT == T_F32 ? 4 : 8) : 1;
+    constexpr int SIZE = DT == T_F32 ? 4 : 2, E = BYTES / SIZE;
+    using V = typename Words<BYTES>::type;
     const int lane = threadIdx.x & 63;
     float s[G];
 #pragma unroll
     for (int j = 0; j < G; ++j) s[j] = 0.0f;
     for (int i = lane * E; i < d; i += 64 * E) {
-        float a[E];
-        if (VEC) {
-            const u32x4 r = *(const u32x4 *)((const unsigned char *)x + (xo + i) * (DT == T_F32 ? 4 : 2));
+        const V a = *(const V *)((const unsigned char *)x + (xo + i) * SIZE);
+        V b[G];
 #pragma unroll
-            for (int e = 0; e < E; ++e) a[e] = load1<DT>(&r, e);
-        } else {
-            a[0] = load1<DT>(x, xo + i);
-        }
-        u32x4 b[G];
-        if (VEC) {
-#pragma unroll
-            for (int j = 0; j < G; ++j) b[j] = *(const u32x4 *)((const unsigned char *)w + (wo[j] + i) * (DT == T_F32 ? 4 : 2));
-        }
+        for (int j = 0; j < G; ++j) b[j] = *(const V *)((const unsigned char *)w + (wo[j] + i) * SIZE);
 #pragma unroll
         for (int j = 0; j < G; ++j)
 #pragma unroll
-            for (int e = 0; e < E; ++e) s[j] = fmaf(a[e], VEC ? load1<DT>(&b[j], e) : load1<DT>(w, wo[j] + i), s[j]);
+            for (int e = 0; e < E; ++e) s[j] = fmaf(load1<DT>(&a, e), load1<DT>(&b[j], e), s[j]);
     }
 #pragma unroll
     for (int o = 32, m = G / 2; m >= 1; o >>= 1, m >>= 1)
@@ -454,7 +460,7 @@ __device__ __forceinline__ float dots(const void *x, const void *w, int64_t xo, 
 
 // LR rows per workgroup (4; 1 where a teacher's rows are few).  The tiles' statistics are read with rows running
 // fastest, then each wave takes whole rows (1 row: its waves share the listed classes).
-template <int DT, bool VEC, int LR>
+template <int DT, int BYTES, int LR>
 __global__ void __launch_bounds__(256) rows_kernel(RowArgs a)
 {
     __shared__ float2 st[256];
@@ -517,7 +523,7 @@ __global__ void __launch_bounds__(256) rows_kernel(RowArgs a)
                     const int64_t id = k0 + j < a.k ? ids[k0 + j] : -1;
                     wo[j] = (alive && id >= 0 ? id : 0) * a.d;            // (a class that is there; its product is not used)
                 }
-                float z = alive ? dots<DT, VEC>(a.x, a.w, r * a.d, wo, a.d) : 0.0f;
+                float z = alive ? dots<DT, BYTES>(a.x, a.w, r * a.d, wo, a.d) : 0.0f;
                 const int k = k0 + ((lane >> 3) & 7);
                 if (k < a.k && (lane & 7) == 0) {
                     float qk = 0.0f;
@@ -790,7 +796,7 @@ Plan make_plan(int64_t n, int64_t v, int d, int dtype)
     p.n = n; p.v = v; p.d = d; p.dtype = dtype;
     p.parts = dtype == T_F32 ? 3 : 1;
     p.dp = (int)up(d, 64);
-    p.direct = dtype != T_F32 && d % 64 == 0;
+    p.direct = dtype != T_F32 && d % 8 == 0;
     p.n_pad = up(n, 256);
     p.small = n <= 32;
     p.quarter = up(n, 256) / 256 * (up(v, 256) / 256) <= CUS;      // (4096 x 1000 x 48 fp32: 26 instead of 44 us of tiles)
@@ -839,6 +845,12 @@ Plan make_plan(int64_t n, int64_t v, int d, int dtype)
     return p;
 }
 
+
+int unit_of(int d, int dtype)
+{
+    const int row = (d * (dtype == T_F32 ? 4 : 2)) | 16;
+    return row & -row;
+}
 
 struct Space {          // hands out 256-byte aligned ranges; with base == NULL only counts
     unsigned char *base;
@@ -958,18 +970,29 @@ void join(const Plan &p, const Join &a, const Join &b, const float *top, float s
     else join_kernel<T_F16><<<g, 256, 0, st>>>(a, b, p.d, p.dp, top, scale);
 }
 
-template <int DT, bool VEC>
+template <int DT, int BYTES>
 void launch_rows(const RowArgs &r, hipStream_t st)
 {
-    if (r.logits == nullptr || r.n >= 2 * CUS) rows_kernel<DT, VEC, 4><<<(unsigned)((r.n + 3) / 4), 256, 0, st>>>(r);
-    else rows_kernel<DT, VEC, 1><<<(unsigned)r.n, 256, 0, st>>>(r);
+    // a teacher's classes are shared by the waves of a workgroup where whole rows would leave the chip idle
+    const bool share = r.logits != nullptr && r.n < (r.k > 16 ? 16 : 2) * CUS;
+    if (share) rows_kernel<DT, BYTES, 1><<<(unsigned)r.n, 256, 0, st>>>(r);
+    else rows_kernel<DT, BYTES, 4><<<(unsigned)((r.n + 3) / 4), 256, 0, st>>>(r);
+}
+template <int DT>
+void launch_rows_of(const RowArgs &r, hipStream_t st)
+{
+    // loads as wide as the rows' alignment allows and no wider than 64 lanes need for a row
+    const int unit = unit_of(r.d, DT), need = (r.d + 63) / 64 * (DT == T_F32 ? 4 : 2);
+    if (unit >= 16 && need > 8) launch_rows<DT, 16>(r, st);
+    else if (unit >= 8 && need > 4) launch_rows<DT, 8>(r, st);
+    else if (unit >= 4 && (need > 2 || DT == T_F32)) launch_rows<DT, 4>(r, st);
+    else launch_rows<DT, DT == T_F32 ? 4 : 2>(r, st);
 }
 void rows_pass(int dtype, const RowArgs &r, hipStream_t st)
 {
-    // 16-byte loads of rows: x and w are aligned, so a row is where its length is
-    if (dtype == T_F32) r.d % 4 == 0 ? launch_rows<T_F32, true>(r, st) : launch_rows<T_F32, false>(r, st);
-    else if (dtype == T_BF16) r.d % 8 == 0 ? launch_rows<T_BF16, true>(r, st) : launch_rows<T_BF16, false>(r, st);
-    else r.d % 8 == 0 ? launch_rows<T_F16, true>(r, st) : launch_rows<T_F16, false>(r, st);
+    if (dtype == T_F32) launch_rows_of<T_F32>(r, st);
+    else if (dtype == T_BF16) launch_rows_of<T_BF16>(r, st);
+    else launch_rows_of<T_F16>(r, st);
 }
 
 const char *bad_head(int64_t n, int64_t v, int d, int dtype, int k, const void *x, const void *w)
@@ -982,7 +1005,8 @@ const char *bad_head(int64_t n, int64_t v, int d, int dtype, int k, const void *
     return nullptr;
 }
 
-Operand rows_of(const void *p, int64_t plane, int64_t ld) { return Operand{(const unsigned short *)p, plane, ld, 0, 0}; }
+// (k: valid elements of a row)
+Operand rows_of(const void *p, int64_t plane, int64_t ld, int64_t k) { return Operand{(const unsigned short *)p, plane, ld, 0, (int)k}; }
 
 const unsigned char *row_ptr(const void *p, int64_t row, int d, int dtype)
 {
@@ -1026,13 +1050,13 @@ int rsdf_class_head_fwd(const void *x, const void *w, int64_t n, int64_t v, int 
         HeadArgs a = {};
         if (!p.direct) {
             PrepArgs r = {};
-            r.d = d; r.dp = p.dp; r.wide = d % (dtype == T_F32 ? 4 : 8) == 0;
+            r.d = d; r.dp = p.dp; r.unit = unit_of(d, dtype);
             if (v0 == 0) add_pack(r, 0, x, n, p.n_pad, f.xp);
             add_pack(r, 1, row_ptr(w, v0, d, dtype), here, p.vf, f.wp);
             prep(dtype, r, st);
         }
-        a.x = p.direct ? rows_of(x, 0, d) : rows_of(f.xp, xplane, p.dp);
-        a.w = p.direct ? rows_of(row_ptr(w, v0, d, dtype), 0, d) : rows_of(f.wp, wplane, p.dp);
+        a.x = p.direct ? rows_of(x, 0, d, d) : rows_of(f.xp, xplane, p.dp, p.dp);
+        a.w = p.direct ? rows_of(row_ptr(w, v0, d, dtype), 0, d, d) : rows_of(f.wp, wplane, p.dp, p.dp);
         a.n = n; a.vc = here;
         a.nseg = p.parts == 3 ? 6 : 1;
         a.depth = p.dp;
@@ -1071,7 +1095,7 @@ int rsdf_class_head_bwd(const void *x, const void *w, int64_t n, int64_t v, int 
         HeadArgs a = {};
         if (v0 == 0 || !p.direct) {
             PrepArgs r = {};
-            r.d = d; r.dp = p.dp; r.wide = d % (dtype == T_F32 ? 4 : 8) == 0;
+            r.d = d; r.dp = p.dp; r.unit = unit_of(d, dtype);
             if (v0 == 0) {
                 r.lse = lse; r.g = grad; r.count = count; r.g_per_row = grad_per_row;
                 r.temperature = temperature; r.n = n;
@@ -1081,8 +1105,8 @@ int rsdf_class_head_bwd(const void *x, const void *w, int64_t n, int64_t v, int 
             if (!p.direct) add_pack(r, 1, row_ptr(w, v0, d, dtype), here, p.vc, b.wp);
             prep(dtype, r, st);
         }
-        a.x = p.direct ? rows_of(x, 0, d) : rows_of(b.xs, xplane, p.dp);
-        a.w = p.direct ? rows_of(row_ptr(w, v0, d, dtype), 0, d) : rows_of(b.wp, wplane, p.dp);
+        a.x = p.direct ? rows_of(x, 0, d, d) : rows_of(b.xs, xplane, p.dp, p.dp);
+        a.w = p.direct ? rows_of(row_ptr(w, v0, d, dtype), 0, d, d) : rows_of(b.wp, wplane, p.dp, p.dp);
         a.n = n; a.n_pad = p.n_pad; a.vc = here; a.ldz = p.vc;
         a.nseg = nseg;
         a.depth = p.dp;
@@ -1104,16 +1128,16 @@ int rsdf_class_head_bwd(const void *x, const void *w, int64_t n, int64_t v, int 
         if (dx != nullptr) {
             px.a = a.w;
             px.a.k_rows = (int)(p.direct ? here : p.vc);
-            px.b = rows_of(b.dz, zplane, p.vc);
+            px.b = rows_of(b.dz, zplane, p.vc, p.vc);
             px.rows = n; px.d = d; px.nseg = nseg;
             px.depth = here;
             px.splits = p.split_dx;
             px.part = b.dxp; px.ldp = p.dp; px.part_stride = n * p.dp; px.add = v0 > 0;
         }
         if (dw != nullptr) {
-            pw.a = rows_of(b.xs, xplane, p.dp);
+            pw.a = rows_of(b.xs, xplane, p.dp, p.dp);
             pw.a.k_rows = (int)p.n_pad;
-            pw.b = rows_of(b.dz, zplane, p.vc);
+            pw.b = rows_of(b.dz, zplane, p.vc, p.vc);
             pw.b.k_rows = (int)p.n_pad;
             pw.rows = here; pw.d = d; pw.nseg = nseg;
             pw.depth = n;

@@ -58,6 +58,16 @@ __device__ __forceinline__ void request16(const unsigned char *base, unsigned of
                  : "memory");
 }
 
+// the same from 64-bit addresses of the lanes' own
+__device__ __forceinline__ void request16_far(const unsigned char *src, unsigned char *dst)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+                 :
+                 : "s"((unsigned)(uintptr_t)(lds_void *)dst), "v"(src)
+                 : "memory");
+}
+__device__ const u32x4 no_k = {0u, 0u, 0u, 0u};       // what rows hold behind their last k
+
 // An operand as the tile sees it: `base` points at its first element (row 0 or column 0 of the tile, k = first k),
 // `ld` in elements.  rows: `lim` = last valid row of the tile's rows (later ones read that row again; their results are
 // not used).  columns: `lim` = last valid column chunk (8 columns), likewise.
@@ -66,7 +76,8 @@ struct Operand {
     int64_t plane;              // elements between the parts of a split fp32 operand
     int64_t ld;
     int lim;
-    int k_rows;                 // columns only: valid k (later ones read the last row again: the other operand is zero there)
+    int k_rows;                 // valid k.  rows: later ones are zero (a multiple of 8); columns: they read the last row again (the
+                                // other operand is zero there)
 };
 
 // the six products of two three-part operands, small ones first: (part of A, part of B)
@@ -120,6 +131,15 @@ struct Loader {
     // request this step into the LDS image `dst`; k_left >= 1: valid k from here on
     __device__ __forceinline__ void issue(unsigned char *dst, int k_left, int wave) const
     {
+        if (!COLS && k_left < KD) {
+#pragma unroll
+            for (int j = 0; j < PER_WAVE; ++j) {
+                const int i = j * WAVES + wave, slot = i * 64 + my_lane(), row = slot / CHUNKS, c = (slot % CHUNKS) ^ swz(row);
+                if (INSTR % WAVES != 0 && i >= INSTR) continue;
+                request16_far(c * 8 < k_left ? cur + off[j] : (const unsigned char *)&no_k, dst + i * 1024);
+            }
+            return;
+        }
         unsigned bo[PER_WAVE];
 #pragma unroll
         for (int j = 0; j < PER_WAVE; ++j) bo[j] = off[j];
