@@ -54,6 +54,19 @@ template <int DT> __device__ __forceinline__ void store1(void *p, int64_t i, flo
     else ((unsigned short *)p)[i] = DT == T_BF16 ? f2bf(v) : f2hf(v);
 }
 
+// vectors at any address of an element (rows of an odd length start anywhere)
+template <class V, int ALIGN> struct __attribute__((packed, aligned(ALIGN))) Anywhere { V v; };
+template <class V, int DT> __device__ __forceinline__ V load_at(const void *p, int64_t i)
+{
+    constexpr int SIZE = DT == T_F32 ? 4 : 2;
+    return ((const Anywhere<V, SIZE> *)((const unsigned char *)p + i * SIZE))->v;
+}
+template <int DT, class V> __device__ __forceinline__ void store_at(void *p, int64_t i, V v)
+{
+    constexpr int SIZE = DT == T_F32 ? 4 : 2;
+    ((Anywhere<V, SIZE> *)((unsigned char *)p + i * SIZE))->v = v;
+}
+
 // three bf16 parts of an fp32 number (an infinity or NaN stays in the first part)
 __device__ __forceinline__ void split3(float v, unsigned short (&h)[3])
 {
@@ -96,7 +109,7 @@ struct Pack { const void *src; int64_t rows, rows_pad; unsigned short *dst; };
 struct PrepArgs {
     Pack p[2];
     int64_t chunks[2];           // 8-element chunks of the two
-    int d, dp, unit;             // unit: bytes, the largest power of two (at most 16) that divides a row
+    int d, dp;
     // weight of a row in the gradient: T g_n (mean: / count), 0 where it takes part in nothing; top[0] = the largest |weight|
     const float *lse, *g, *count;
     int g_per_row;
@@ -137,20 +150,10 @@ __global__ void __launch_bounds__(PREP) prep_kernel(PrepArgs a)
         bool live = r < p.rows;
         if (live && !second && a.lse != nullptr) live = a.lse[r] != __builtin_inff() && a.g[a.g_per_row ? r : 0] != 0.0f;
         float x[8];
-        if (live && c + 8 <= a.d && (DT != T_F32 ? a.unit >= 4 : a.unit >= 8)) {        // (rows start at multiples of the unit)
-            const unsigned char *s = (const unsigned char *)p.src + (r * a.d + c) * (DT == T_F32 ? 4 : 2);
-            unsigned raw[8];
-            constexpr int WORDS = DT == T_F32 ? 8 : 4;
-            if (a.unit == 16) {
-#pragma unroll
-                for (int i = 0; i < WORDS; i += 4) *(u32x4 *)(raw + i) = *(const u32x4 *)(s + 4 * i);
-            } else if (a.unit == 8) {
-#pragma unroll
-                for (int i = 0; i < WORDS; i += 2) *(uint2 *)(raw + i) = *(const uint2 *)(s + 4 * i);
-            } else {
-#pragma unroll
-                for (int i = 0; i < WORDS; ++i) raw[i] = *(const unsigned *)(s + 4 * i);
-            }
+        if (live && c + 8 <= a.d) {
+            u32x4 raw[2];
+            raw[0] = load_at<u32x4, DT>(p.src, r * a.d + c);
+            if (DT == T_F32) raw[1] = load_at<u32x4, DT>(p.src, r * a.d + c + 4);
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[e] = load1<DT>(raw, e);
         } else {
@@ -426,25 +429,31 @@ constexpr int G = 8;
 template <int E> struct Words { using type = u32x4; };
 template <> struct Words<8> { using type = uint2; };
 template <> struct Words<4> { using type = unsigned; };
-template <> struct Words<2> { using type = unsigned short; };
 template <int DT, int BYTES>
 __device__ __forceinline__ float dots(const void *x, const void *w, int64_t xo, const int64_t (&wo)[G], int d)
 {
-    constexpr int SIZE = DT == T_F32 ? 4 : 2, E = BYTES / SIZE;
+    constexpr int E = BYTES / (DT == T_F32 ? 4 : 2);
     using V = typename Words<BYTES>::type;
     const int lane = threadIdx.x & 63;
     float s[G];
 #pragma unroll
     for (int j = 0; j < G; ++j) s[j] = 0.0f;
-    for (int i = lane * E; i < d; i += 64 * E) {
-        const V a = *(const V *)((const unsigned char *)x + (xo + i) * SIZE);
+    int i = lane * E;
+    for (; i + E <= d; i += 64 * E) {
+        const V a = load_at<V, DT>(x, xo + i);
         V b[G];
 #pragma unroll
-        for (int j = 0; j < G; ++j) b[j] = *(const V *)((const unsigned char *)w + (wo[j] + i) * SIZE);
+        for (int j = 0; j < G; ++j) b[j] = load_at<V, DT>(w, wo[j] + i);
 #pragma unroll
         for (int j = 0; j < G; ++j)
 #pragma unroll
             for (int e = 0; e < E; ++e) s[j] = fmaf(load1<DT>(&a, e), load1<DT>(&b[j], e), s[j]);
+    }
+    i = d / E * E + lane;
+    if (E > 1 && i < d) {
+        const float a = load1<DT>(x, xo + i);
+#pragma unroll
+        for (int j = 0; j < G; ++j) s[j] = fmaf(a, load1<DT>(w, wo[j] + i), s[j]);
     }
 #pragma unroll
     for (int o = 32, m = G / 2; m >= 1; o >>= 1, m >>= 1)
@@ -660,7 +669,6 @@ __device__ __forceinline__ void product(const ProdArgs &a, int64_t job, unsigned
     TL::run(acc, A, B, a.nseg, ksteps, s0, s1, lds);
 
     const float f = a.part == nullptr ? a.top[0] * a.scale : 1.0f;
-    const bool wide = (a.d & 7) == 0;
 #pragma unroll
     for (int nt = 0; nt < TL::NT; ++nt) {
         const int64_t n = n0 + TL::n_of(nt);
@@ -683,28 +691,26 @@ __device__ __forceinline__ void product(const ProdArgs &a, int64_t job, unsigned
                 }
                 continue;
             }
-            if (wide) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    if (m + 8 * h >= a.d) continue;
-                    float v[8];
+            for (int h = 0; h < 2; ++h) {
+                const int64_t at = m + 8 * h, to = n * a.d + at;
+                if (at >= a.d) continue;
+                float v[8];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] = TL::quad(acc, b, 2 * h + (e >> 2), nt)[e & 3] * f;
-                    if (DT == T_F32) {
-                        float4 *o = (float4 *)((float *)a.out + n * a.d + m + 8 * h);
-                        o[0] = float4{v[0], v[1], v[2], v[3]};
-                        o[1] = float4{v[4], v[5], v[6], v[7]};
-                    } else {
-                        unsigned short u[8];
+                for (int e = 0; e < 8; ++e) v[e] = TL::quad(acc, b, 2 * h + (e >> 2), nt)[e & 3] * f;
+                if (at + 8 > a.d) {
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) u[e] = to16<DT == T_F16>(v[e]);
-                        *(u32x4 *)((unsigned short *)a.out + n * a.d + m + 8 * h) = *(const u32x4 *)u;
-                    }
+                    for (int e = 0; e < 7; ++e)
+                        if (at + e < a.d) store1<DT>(a.out, to + e, v[e]);
+                } else if (DT == T_F32) {
+                    store_at<DT>(a.out, to, f32x4{v[0], v[1], v[2], v[3]});
+                    store_at<DT>(a.out, to + 4, f32x4{v[4], v[5], v[6], v[7]});
+                } else {
+                    unsigned short u[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) u[e] = to16<DT == T_F16>(v[e]);
+                    store_at<DT>(a.out, to, *(const u32x4 *)u);
                 }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    if (m + e < a.d) store1<DT>(a.out, n * a.d + m + e, TL::quad(acc, b, e >> 2, nt)[e & 3] * f);
             }
         }
     }
@@ -760,18 +766,16 @@ __global__ void __launch_bounds__(256) join_kernel(Join ja, Join jb, int d, int6
             }
         }
         const float v[4] = {s.x * g, s.y * g, s.z * g, s.w * g};
-        if ((d & 3) == 0) {
-            if (DT == T_F32) {
-                *(float4 *)((float *)a.out + r * d + c) = float4{v[0], v[1], v[2], v[3]};
-            } else {
-                unsigned short u[4];
-                for (int e = 0; e < 4; ++e) u[e] = to16<DT == T_F16>(v[e]);
-                *(uint2 *)((unsigned short *)a.out + r * d + c) = *(const uint2 *)u;
-            }
-            continue;
+        if (c + 4 > d) {
+            for (int e = 0; e < 3; ++e)
+                if (c + e < d) store1<DT>(a.out, r * d + c + e, v[e]);
+        } else if (DT == T_F32) {
+            store_at<DT>(a.out, r * d + c, f32x4{v[0], v[1], v[2], v[3]});
+        } else {
+            unsigned short u[4];
+            for (int e = 0; e < 4; ++e) u[e] = to16<DT == T_F16>(v[e]);
+            store_at<DT>(a.out, r * d + c, *(const unsigned long long *)u);
         }
-        for (int e = 0; e < 4; ++e)
-            if (c + e < d) store1<DT>(a.out, r * d + c + e, v[e]);
     }
 }
 
@@ -845,12 +849,6 @@ Plan make_plan(int64_t n, int64_t v, int d, int dtype)
     return p;
 }
 
-
-int unit_of(int d, int dtype)
-{
-    const int row = (d * (dtype == T_F32 ? 4 : 2)) | 16;
-    return row & -row;
-}
 
 struct Space {          // hands out 256-byte aligned ranges; with base == NULL only counts
     unsigned char *base;
@@ -981,12 +979,11 @@ void launch_rows(const RowArgs &r, hipStream_t st)
 template <int DT>
 void launch_rows_of(const RowArgs &r, hipStream_t st)
 {
-    // loads as wide as the rows' alignment allows and no wider than 64 lanes need for a row
-    const int unit = unit_of(r.d, DT), need = (r.d + 63) / 64 * (DT == T_F32 ? 4 : 2);
-    if (unit >= 16 && need > 8) launch_rows<DT, 16>(r, st);
-    else if (unit >= 8 && need > 4) launch_rows<DT, 8>(r, st);
-    else if (unit >= 4 && (need > 2 || DT == T_F32)) launch_rows<DT, 4>(r, st);
-    else launch_rows<DT, DT == T_F32 ? 4 : 2>(r, st);
+    // loads no wider than 64 lanes need for a row
+    const int need = (r.d + 63) / 64 * (DT == T_F32 ? 4 : 2);
+    if (need > 8) launch_rows<DT, 16>(r, st);
+    else if (need > 4) launch_rows<DT, 8>(r, st);
+    else launch_rows<DT, 4>(r, st);
 }
 void rows_pass(int dtype, const RowArgs &r, hipStream_t st)
 {
@@ -1050,7 +1047,7 @@ int rsdf_class_head_fwd(const void *x, const void *w, int64_t n, int64_t v, int 
         HeadArgs a = {};
         if (!p.direct) {
             PrepArgs r = {};
-            r.d = d; r.dp = p.dp; r.unit = unit_of(d, dtype);
+            r.d = d; r.dp = p.dp;
             if (v0 == 0) add_pack(r, 0, x, n, p.n_pad, f.xp);
             add_pack(r, 1, row_ptr(w, v0, d, dtype), here, p.vf, f.wp);
             prep(dtype, r, st);
@@ -1095,7 +1092,7 @@ int rsdf_class_head_bwd(const void *x, const void *w, int64_t n, int64_t v, int 
         HeadArgs a = {};
         if (v0 == 0 || !p.direct) {
             PrepArgs r = {};
-            r.d = d; r.dp = p.dp; r.unit = unit_of(d, dtype);
+            r.d = d; r.dp = p.dp;
             if (v0 == 0) {
                 r.lse = lse; r.g = grad; r.count = count; r.g_per_row = grad_per_row;
                 r.temperature = temperature; r.n = n;
