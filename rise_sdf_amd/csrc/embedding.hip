@@ -35,50 +35,59 @@ template <> struct Elem<T_F16> {
     __device__ static __forceinline__ float get(unsigned short v) { return (float)__builtin_bit_cast(_Float16, v); }
     __device__ static __forceinline__ unsigned short put(float v) { return __builtin_bit_cast(unsigned short, (_Float16)v); }
 };
-template <class T, int N> struct alignas(sizeof(T) * N) Vec { T v[N]; };
-
-// a store that does not stay in the caches: written once, read by someone else
-template <class V>
-__device__ __forceinline__ void nt_store(V *p, const V &v)
+// N elements at any address of an element: rows of an odd length start anywhere, and the last vector of a row begins where it
+// ends with the row (what it shares with the one before is handled twice, alike)
+template <class T, int N> struct Vec { T v[N]; };
+template <int BYTES> struct Bits { using type = __attribute__((ext_vector_type(BYTES / 4))) unsigned; };
+template <> struct Bits<4> { using type = unsigned; };
+template <> struct Bits<2> { using type = unsigned short; };
+template <class V> __device__ __forceinline__ int element_of(int c, int d)
 {
-    if constexpr (sizeof(V) == 16) {
-        using B = __attribute__((ext_vector_type(4))) unsigned;
-        __builtin_nontemporal_store(*(const B *)&v, (B *)p);
-    } else if constexpr (sizeof(V) == 8) {
-        using B = __attribute__((ext_vector_type(2))) unsigned;
-        __builtin_nontemporal_store(*(const B *)&v, (B *)p);
-    } else {
-        *p = v;
-    }
+    constexpr int N = sizeof(V) / sizeof(V::v[0]);
+    return c * N + N <= d ? c * N : d - N;
+}
+template <class V, class T> __device__ __forceinline__ V load_at(const T *p, int64_t i)
+{
+    typedef typename Bits<sizeof(V)>::type B __attribute__((aligned(sizeof(T))));
+    return __builtin_bit_cast(V, *(const B *)(p + i));
+}
+// NT: a store that does not stay in the caches: written once, read by someone else
+template <bool NT, class V, class T> __device__ __forceinline__ void store_at(T *p, int64_t i, const V &v)
+{
+    typedef typename Bits<sizeof(V)>::type B __attribute__((aligned(sizeof(T))));
+    if (NT && sizeof(V) >= 8) __builtin_nontemporal_store(__builtin_bit_cast(typename Bits<sizeof(V)>::type, v), (B *)(p + i));
+    else *(B *)(p + i) = __builtin_bit_cast(typename Bits<sizeof(V)>::type, v);
 }
 
 // ---- lookup -------------------------------------------------------------------------------------------------------------------
 // NT: the output passes the caches by (262144 x 256 bf16: 28 instead of 42 us, and the table stays in them)
 template <int DT, int VW, bool NT>
 __global__ void __launch_bounds__(256) lookup_kernel(const int64_t *__restrict__ ids, int64_t n, const void *__restrict__ table, int64_t v,
-                                                     int per_row, float scale, int64_t padding, int rows_per_block,
+                                                     int d, int per_row, float scale, int64_t padding, int rows_per_block,
                                                      void *__restrict__ out, int *__restrict__ bad_ids)
 {
     using E = Elem<DT>;
-    using V = Vec<typename E::type, VW>;
+    using T = typename E::type;
+    using V = Vec<T, VW>;
     constexpr int U = 4;
     const int64_t r0 = (int64_t)blockIdx.x * rows_per_block;
     const int rows = (int)(n - r0 < rows_per_block ? n - r0 : rows_per_block), items = rows * per_row;
     for (int i0 = threadIdx.x; i0 < items; i0 += 256 * U) {
         int64_t id[U];
-        int c[U];
+        int c[U], to[U];
         V o[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int i = i0 + u * 256 < items ? i0 + u * 256 : i0;
             const int r = i / per_row;
-            c[u] = i - r * per_row;
+            c[u] = element_of<V>(i - r * per_row, d);
+            to[u] = r * d + c[u];
             id[u] = ids[r0 + r];
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const bool in = id[u] >= 0 && id[u] < v;
-            o[u] = ((const V *)table)[(in ? id[u] : 0) * per_row + c[u]];
+            o[u] = load_at<V>((const T *)table, (in ? id[u] : 0) * d + c[u]);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -90,8 +99,7 @@ __global__ void __launch_bounds__(256) lookup_kernel(const int64_t *__restrict__
                 o[u].v[e] = E::put(id[u] == padding ? 0.0f : f);
             }
             if (!in && id[u] != padding && c[u] == 0 && bad_ids != nullptr) atomicAdd(bad_ids, 1);
-            if (NT) nt_store((V *)out + r0 * per_row + i0 + u * 256, o[u]);
-            else ((V *)out)[r0 * per_row + i0 + u * 256] = o[u];
+            store_at<NT>((T *)out + r0 * d, to[u], o[u]);
         }
     }
 }
@@ -209,16 +217,18 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_scatter_kernel(const int64_
 // ---- few positions: no list -----------------------------------------------------------------------------------------------------
 // One wave per row of the table walks all ids, 64 at a time, and adds up its positions in order: one launch, no workspace.
 template <int DT, int VW>
-__global__ void __launch_bounds__(256) few_kernel(const int64_t *__restrict__ ids, int n, const void *__restrict__ g, int64_t v, int per_row,
+__global__ void __launch_bounds__(256) few_kernel(const int64_t *__restrict__ ids, int n, const void *__restrict__ g, int64_t v, int d, int per_row,
                                                   float scale, int64_t padding, void *__restrict__ out)
 {
     using E = Elem<DT>;
-    using V = Vec<typename E::type, VW>;
+    using T = typename E::type;
+    using V = Vec<T, VW>;
     const int lane = threadIdx.x & 63;
     const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (row >= v) return;
     for (int c = lane; c - lane < per_row; c += 64) {
         float acc[VW];
+        const int col = element_of<V>(c < per_row ? c : 0, d);
 #pragma unroll
         for (int k = 0; k < VW; ++k) acc[k] = 0.0f;
         for (int i0 = 0; i0 < n; i0 += 64) {
@@ -234,7 +244,7 @@ __global__ void __launch_bounds__(256) few_kernel(const int64_t *__restrict__ id
                     const int at = i0 + __ffsll((long long)m) - 1;
                     m &= m - 1;
                     here = u + 1;
-                    x[u] = ((const V *)g)[(int64_t)at * per_row + (c < per_row ? c : 0)];
+                    x[u] = load_at<V>((const T *)g, (int64_t)at * d + col);
                 }
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
@@ -248,7 +258,7 @@ __global__ void __launch_bounds__(256) few_kernel(const int64_t *__restrict__ id
             V o;
 #pragma unroll
             for (int k = 0; k < VW; ++k) o.v[k] = E::put(acc[k] * scale);
-            ((V *)out)[row * per_row + c] = o;
+            store_at<false>((T *)out, row * d + col, o);
         }
     }
 }
@@ -258,7 +268,7 @@ constexpr int LONG = 16;         // a run over more chunks than this is joined b
 struct SumArgs {
     const unsigned *keys, *pos;
     int64_t n, v;
-    int d, per_row;              // row length in elements / in vectors
+    int d, per_row;              // row length in elements / in vectors (the last one may overlap)
     int chunk;
     int64_t chunks;
     const void *g;
@@ -275,7 +285,8 @@ template <int DT, int VW>
 __global__ void __launch_bounds__(256) sum_kernel(SumArgs a)
 {
     using E = Elem<DT>;
-    using V = Vec<typename E::type, VW>;
+    using T = typename E::type;
+    using V = Vec<T, VW>;
     constexpr int U = 4;
     if ((int64_t)blockIdx.x >= a.sum_blocks) {
         // rows without a position
@@ -297,14 +308,14 @@ __global__ void __launch_bounds__(256) sum_kernel(SumArgs a)
         V z = {};
         for (int i = threadIdx.x; i < rows * a.per_row; i += 256) {
             const int r = i / a.per_row;
-            if (absent[r]) ((V *)a.out)[r0 * a.per_row + i] = z;
+            if (absent[r]) store_at<false>((T *)a.out + r0 * a.d, r * a.d + element_of<V>(i - r * a.per_row, a.d), z);
         }
         return;
     }
     const int group = threadIdx.x / a.lanes, l = threadIdx.x % a.lanes;
     const int64_t c = (int64_t)blockIdx.x * a.groups + group;
-    const int col = blockIdx.y * a.lanes + l;
-    if (c >= a.chunks || col >= a.per_row) return;
+    const int vec = blockIdx.y * a.lanes + l, col = element_of<V>(vec, a.d);
+    if (c >= a.chunks || vec >= a.per_row) return;
     const int64_t b = c * a.chunk, e = b + a.chunk < a.n ? b + a.chunk : a.n;
     const unsigned none = (unsigned)a.v;
     const unsigned prev = b > 0 ? a.keys[b - 1] : none, next = e < a.n ? a.keys[e] : none;
@@ -320,12 +331,12 @@ __global__ void __launch_bounds__(256) sum_kernel(SumArgs a)
             V o;
 #pragma unroll
             for (int k = 0; k < VW; ++k) o.v[k] = E::put(acc[k] * a.scale);
-            ((V *)a.out)[(int64_t)cur * a.per_row + col] = o;
+            store_at<false>((T *)a.out, (int64_t)cur * a.d + col, o);
         } else {
-            float *p = a.part + (c * 2 + (head ? 0 : 1)) * a.d + col * VW;
+            float *p = a.part + (c * 2 + (head ? 0 : 1)) * a.d + col;
 #pragma unroll
             for (int k = 0; k < VW; ++k) p[k] = acc[k];
-            if (!head && col == 0) {
+            if (!head && vec == 0) {
                 const int64_t far = b + (int64_t)a.chunk * (LONG + 1);
                 a.goes_on[c] = far < a.n && a.keys[far] == cur ? 2 : 1;
                 marked = true;
@@ -339,7 +350,7 @@ __global__ void __launch_bounds__(256) sum_kernel(SumArgs a)
         for (int u = 0; u < U; ++u) {
             const int64_t j = i + u < e ? i + u : e - 1;
             key[u] = a.keys[j];
-            row[u] = ((const V *)a.g)[(int64_t)a.pos[j] * a.per_row + col];
+            row[u] = load_at<V>((const T *)a.g, (int64_t)a.pos[j] * a.d + col);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -356,7 +367,7 @@ __global__ void __launch_bounds__(256) sum_kernel(SumArgs a)
         }
     }
     flush(true);
-    if (!marked && col == 0) a.goes_on[c] = 0;
+    if (!marked && vec == 0) a.goes_on[c] = 0;
 }
 
 // The runs that cross chunks: one wave per chunk and 64 columns looks whether one begins there.  A short run it joins by itself, a
@@ -466,12 +477,13 @@ const char *bad_shape(int64_t n, int64_t v, int d, int dtype)
     return nullptr;
 }
 
-// bytes of a vector that divides a row of d elements and the addresses
-int vector_bytes(int d, int dtype, const void *p, const void *q)
+// bytes of a vector: 16, less only where a row is shorter
+int vector_bytes(int d, int dtype)
 {
-    const uintptr_t row = (uintptr_t)d * (dtype == T_F32 ? 4 : 2);
-    const uintptr_t all = row | (uintptr_t)p | (uintptr_t)q | 16;
-    return (int)(all & (~all + 1));
+    const int size = dtype == T_F32 ? 4 : 2;
+    int bytes = 16;
+    while (bytes > d * size) bytes /= 2;
+    return bytes;
 }
 
 }  // namespace
@@ -504,15 +516,15 @@ int rsdf_embedding_fwd(const int64_t *ids, int64_t n, const void *table, int64_t
     const char *bad = bad_shape(n, v, d, dtype);
     RSDF_CHECK_ARG(bad == nullptr, bad);
     if (n == 0) return 0;
-    const int bytes = vector_bytes(d, dtype, table, out);
-    const int per_row = d * (dtype == T_F32 ? 4 : 2) / bytes;
+    const int bytes = vector_bytes(d, dtype), size = dtype == T_F32 ? 4 : 2;
+    const int per_row = (d * size + bytes - 1) / bytes;
     int rows = 1024 / per_row;                          // about four vectors a thread
     rows = rows < 1 ? 1 : rows;
     const unsigned grid = (unsigned)((n + rows - 1) / rows);
-    const bool past = n * d * (dtype == T_F32 ? 4 : 2) >= L2_BYTES;
+    const bool past = n * d * size >= L2_BYTES;
 #define CALL(DT, VW)                                                                                                                   \
-    past ? lookup_kernel<DT, VW, true><<<grid, 256, 0, (hipStream_t)stream>>>(ids, n, table, v, per_row, scale, padding_id, rows, out, bad_ids) \
-         : lookup_kernel<DT, VW, false><<<grid, 256, 0, (hipStream_t)stream>>>(ids, n, table, v, per_row, scale, padding_id, rows, out, bad_ids)
+    past ? lookup_kernel<DT, VW, true><<<grid, 256, 0, (hipStream_t)stream>>>(ids, n, table, v, d, per_row, scale, padding_id, rows, out, bad_ids) \
+         : lookup_kernel<DT, VW, false><<<grid, 256, 0, (hipStream_t)stream>>>(ids, n, table, v, d, per_row, scale, padding_id, rows, out, bad_ids)
     RSDF_EMBEDDING_DISPATCH(dtype, bytes, CALL);
 #undef CALL
     RSDF_RETURN_LAUNCH();
@@ -531,10 +543,10 @@ int rsdf_embedding_bwd(const int64_t *ids, int64_t n, const void *grad, int64_t 
     const char *bad = bad_shape(n, v, d, dtype);
     RSDF_CHECK_ARG(bad == nullptr, bad);
     hipStream_t st = (hipStream_t)stream;
-    const int bytes = vector_bytes(d, dtype, grad, d_table);
-    const int per_row = d * (dtype == T_F32 ? 4 : 2) / bytes;
+    const int bytes = vector_bytes(d, dtype), size = dtype == T_F32 ? 4 : 2;
+    const int per_row = (d * size + bytes - 1) / bytes;
     if (use_few(n, v)) {
-#define CALL(DT, VW) few_kernel<DT, VW><<<(unsigned)((v + 3) / 4), 256, 0, st>>>(ids, (int)n, grad, v, per_row, scale, padding_id, d_table)
+#define CALL(DT, VW) few_kernel<DT, VW><<<(unsigned)((v + 3) / 4), 256, 0, st>>>(ids, (int)n, grad, v, d, per_row, scale, padding_id, d_table)
         RSDF_EMBEDDING_DISPATCH(dtype, bytes, CALL);
 #undef CALL
         RSDF_RETURN_LAUNCH();

@@ -179,17 +179,17 @@ __device__ __forceinline__ u32x4 fragment(const unsigned char *img, int tile16, 
     return u32x4{(unsigned)l, (unsigned)(l >> 32), (unsigned)h, (unsigned)(h >> 32)};
 }
 
-template <int BM_, int BN_, int WM_, int WN_, bool ACOLS_, bool BCOLS_, bool F16_>
+template <int BM_, int BN_, int WM_, int WN_, bool ACOLS_, bool BCOLS_, bool F16_, int STAGES_ = 3>
 struct Tile {
     static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;             // waves along m and n
     static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
-        static constexpr int KD = BK, STAGES = 3;                                // depth of a step, steps in LDS
-    static constexpr int OCCUPANCY = 2 * WAVES / 4;                          // waves per SIMD: two workgroups per CU
+    static constexpr int KD = BK, STAGES = STAGES_;                          // depth of a step, steps in LDS
     static constexpr bool ACOLS = ACOLS_, BCOLS = BCOLS_, F16 = F16_;
     static constexpr int TM = BM / WM, TN = BN / WN;                         // per wave
     static constexpr int MT = TM / 16, NT = TN / 16;
     static constexpr int A_BYTES = BM * KD * 2, B_BYTES = BN * KD * 2, STAGE = A_BYTES + B_BYTES;
     static constexpr int LDS = STAGES * STAGE;
+    static constexpr int OCCUPANCY = (LDS > 80 * 1024 ? 1 : 2) * WAVES / 4;  // waves per SIMD: one or two workgroups per CU
     using LA = Loader<ACOLS, BM, true, WAVES, KD>;
     using LB = Loader<BCOLS, BN, BCOLS, WAVES, KD>;
     static_assert(TM % 64 == 0, "a wave holds whole permuted blocks");
@@ -223,6 +223,18 @@ struct Tile {
         asm volatile("" ::: "memory");
     }
 
+    // with `later` steps requested behind this one
+    template <int N, int PER>
+    __device__ static __forceinline__ void tail_sync(int later)
+    {
+        if constexpr (N > 0) {
+            if (later >= N) sync<N * PER>();
+            else tail_sync<N - 1, PER>(later);
+        } else {
+            sync<0>();
+        }
+    }
+
     // steps [s0, s1) of the nseg * ksteps steps
     __device__ static __forceinline__ void run(Acc &acc, const Operand &A, const Operand &Bo, int nseg, int64_t ksteps, int64_t s0,
                                                int64_t s1, unsigned char *lds)
@@ -254,9 +266,10 @@ struct Tile {
                 }
             }
         };
-        // requests of one step by this wave (0: not the same for every wave)
-        constexpr int PER = LA::INSTR % WAVES == 0 && LB::INSTR % WAVES == 0 ? LA::PER_WAVE + LB::PER_WAVE : 0;
+        // requests of one step by the wave that has the fewest (the others wait for a few more than they must)
+        constexpr int PER = LA::INSTR / WAVES + LB::INSTR / WAVES;
         constexpr int DEPTH = STAGES - 1;         // steps requested ahead
+        static_assert((DEPTH - 1) * PER < 64, "vmcnt has six bits");
         const int pre = steps < DEPTH ? steps : DEPTH;
         for (int i = 0; i < pre; ++i) request();
         // step s has arrived when only the later steps' requests are outstanding; lgkmcnt(0): this wave's reads of the image that
@@ -272,8 +285,7 @@ struct Tile {
             get = get == lds + (STAGES - 1) * STAGE ? lds : get + STAGE;
         }
         for (; s < steps; ++s) {
-            if (s + DEPTH - 1 < steps) sync<(DEPTH - 1) * PER>();
-            else sync<0>();
+            tail_sync<DEPTH - 1, PER>(steps - 1 - s);
             read(f, get, wm, wn, lane);
             multiply(acc, f);
             get = get == lds + (STAGES - 1) * STAGE ? lds : get + STAGE;
