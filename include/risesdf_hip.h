@@ -732,8 +732,8 @@ int rsdf_embedding_bwd(const int64_t *ids, int64_t n, const void *grad, int64_t 
  *   least 1); 2: loss [1] = sum.  lse [n], q [n][k] and listed_z [n][k] (teacher only) are what bwd reads.
  * bwd: grad = d(loss): [n] (grad_per_row) or [1]; count as written by fwd for reduction 1, else NULL.  dx [n][d] / dw [v][d]
  *   (nullable: not computed).
- * workspace: >= rsdf_class_head_workspace_bytes(n, v, d, dtype, pass), pass 0 forward, else backward (1 dx, 2 dw, 3 both);
- * its size does not grow with n * v. */
+ * workspace: >= rsdf_class_head_workspace_bytes(n, v, d, dtype, pass), pass 0 forward, else backward (1 dx, 2 dw, 3 both): the
+ * forward's holds 8 bytes per row and 256 (few tiles: 128) classes, the backward's one piece of the classes, 128 MB or 256 classes. */
 int64_t rsdf_class_head_workspace_bytes(int64_t n, int64_t v, int d, int dtype, int pass);
 int rsdf_class_head_fwd(const void *x, const void *w, int64_t n, int64_t v, int d, int dtype, const int64_t *ids,
                         const float *teacher_logits /*nullable*/, int k, int64_t ignore_id, float temperature, int reduction,

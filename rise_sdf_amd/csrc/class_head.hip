@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(PREP) prep_kernel(PrepArgs a)
         for (int64_t i = threadIdx.x; i < a.n; i += PREP) {
             const float wr = a.lse[i] != __builtin_inff() ? a.g[a.g_per_row ? i : 0] * f : 0.0f;
             a.weight[i] = wr;
-            m = fmaxf(m, fabsf(wr));
+            m = fmaxf(m, fabsf(wr) < __builtin_inff() ? fabsf(wr) : 0.0f);      // (an infinite or NaN one spoils its own row)
         }
         m = wave_max(m);
         if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = m;

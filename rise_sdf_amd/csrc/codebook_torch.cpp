@@ -4,6 +4,7 @@
 // librisesdf_hip.so come in as addresses (bind), so that this module works with whichever build of the library is loaded.
 // Host code only: no kernels here.
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -49,6 +50,22 @@ Tensor bytes_on(int64_t n, const Tensor &like)
 }
 
 template <class T> T *address(const Tensor &t) { return t.defined() ? (T *)t.data_ptr() : nullptr; }
+
+// A leaf remembers the stream on which a graph that is still alive first used it, and its gradient is accumulated there.  Inside a
+// capture that would tie an eager stream to the captured one, which ends the process, so the call is refused while it can be.
+void check_leaf(const Tensor &t, const char *what)
+{
+    if (!at::GradMode::is_enabled() || !t.requires_grad() || !t.is_leaf()) return;
+    const c10::DeviceGuard guard(t.device());
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+    if (node == nullptr) return;
+    const auto there = node->stream();
+    // (by id: one of the two calls the device HIP, the other CUDA)
+    if (there.has_value() && there->id() != c10::hip::getCurrentHIPStream(t.get_device()).id())
+        throw Error(std::string(what) + ": a leaf of this captured pass is part of a graph that was recorded on another stream and is "
+                    "still alive; drop that graph (its outputs and losses) before the capture");
+}
 
 // gradients of a node that cannot be differentiated again: under create_graph a second derivative raises instead of being zero
 variable_list once(variable_list grads, const char *what)
@@ -196,11 +213,14 @@ PYBIND11_MODULE(_codebook, m)
     m.def("bind", &bind);
     m.def("embedding", [](const Tensor &ids, const Tensor &table, double scale, int64_t padding, int64_t bad_ids) {
         py::gil_scoped_release free;
+        check_leaf(table, "embedding");
         return Embedding::apply(ids, table, scale, padding, bad_ids);
     });
     m.def("class_head", [](const Tensor &x, const Tensor &w, const Tensor &ids, const c10::optional<Tensor> &logits, int64_t k, int64_t ignore,
                            double temperature, int64_t reduction, int64_t bad_ids) {
         py::gil_scoped_release free;
+        check_leaf(x, "the losses of a linear head");
+        check_leaf(w, "the losses of a linear head");
         return ClassHead::apply(x, w, ids, logits, k, ignore, temperature, reduction, bad_ids);
     });
 }

@@ -164,7 +164,8 @@ def linear_cross_entropy(x, weight, target, *, ignore_index=-100, reduction="mea
 
     ``x`` [..., D], ``weight`` [V, D] of one type (fp32: fp32-equivalent split products; bf16 / fp16: fp32 sums), ``target``
     [...] integers.  ``reduction``: "none" -> [...], "mean" over the rows that are not ignored (0 if all are), "sum"; fp32.
-    Differentiable w.r.t. ``x`` and ``weight`` (once).  Rows with ``target == ignore_index`` take part in nothing, whatever
+    Differentiable w.r.t. ``x`` and ``weight`` (once); a pass may be captured into a graph, but not while an eager graph of the
+    same leaf is alive (refused).  Rows with ``target == ignore_index`` take part in nothing, whatever
     ``x`` holds there; any other target outside [0, V) makes its row NaN, takes no part in the gradients and is reported by
     ``rise_sdf_amd.check_status()``."""
     if target.shape != x.shape[:-1]:

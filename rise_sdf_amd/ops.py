@@ -731,7 +731,8 @@ def embedding(ids, table, scale=1.0, padding_idx=None):
 
     Differentiable w.r.t. ``table`` (a dense gradient, summed in fp32 by sorted ids: the same bits every time).  An id outside
     [0, V) (negative ones too: they do not wrap) gives a row of NaN, takes no part in the gradient and is reported by
-    ``rise_sdf_amd.check_status()`` and by the samplers' own polls."""
+    ``rise_sdf_amd.check_status()`` and by the samplers' own polls.  A pass may be captured into a graph, but not while an
+    eager graph of the same table, recorded on another stream, is alive (refused)."""
     if not torch.is_tensor(table) or table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1:
         raise L.RiseSdfHipError("embedding: table must be [V, D] with V, D >= 1")
     _dtype_id(table, "embedding")
