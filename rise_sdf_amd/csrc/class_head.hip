@@ -32,7 +32,9 @@ constexpr int T_F32 = 0, T_BF16 = 1, T_F16 = 2;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float F16_DZ = 4096.0f;
 constexpr int64_t DZ_BYTES = 128ll << 20;      // of one piece of dz
-constexpr double JOB_STEPS = 6.0;                // of a job of the products beyond its own steps
+// us of a step (64 deep) of a job of the products, and steps that a job costs beyond its own.  With 256 x 256 tiles alone 1000 x 10000 x
+// 200 bf16 took 90 us (here 76), with 128 x 128 ones 4096 x 32768 x 512 607 us (here 558); 0.45 to 0.65 chose alike but for long rows.
+constexpr double STEP_256 = 1.0, STEP_128 = 0.57, JOB_STEPS = 6.0;
 constexpr int CUS = 256;                        // MI355X
 constexpr int64_t WPACK_BYTES = 128ll << 20;   // of the packed class codes of one piece
 
@@ -784,15 +786,26 @@ int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
 
 struct Plan {
     int sbm;                         // classes of a forward tile
-    bool quarter;                    // few tiles: 128 x 128 ones
+    bool quarter_fwd, quarter_bwd;   // z by 128 x 128 tiles
     int64_t n, v, n_pad, vf, vc;     // vf, vc: classes of a piece, forward and backward (whole piece stride)
     int d, dp, parts, dtype;
     bool direct;                     // operands are read where they are
     bool small;                      // few rows: tiles of 32 rows
-    int bm;                          // width of the d side of the products' tiles
+    int bm;                          // the products' tiles are bm x bm
     int split_dx, split_dw;
     bool x_first;                    // the jobs of dx are the longer ones
 };
+
+// Tiles of z: 256 x 256, one per CU, or 128 x 128, two per CU.  Estimated us of a launch from what steps (64 deep) and results of a tile
+// took: the large ones come in whole rounds, the small ones fill the last one better (1000 x 20000 x 256 bf16: forward 18.4 against 22.9
+// us with large ones, backward 24.6 and 30.5; 1000 x 3000 x 100 fp32 11.2 and 21.4; but 4096 x 4096 x 256 fp32 57.5 and 40.8).
+bool by_quarters(int64_t n, int64_t classes, int64_t steps)
+{
+    const int64_t large = (n + 255) / 256 * ((classes + 255) / 256), small = (n + 127) / 128 * ((classes + 127) / 128);
+    const double t256 = (double)((large + CUS - 1) / CUS) * (1.4 * steps + 5.0);
+    const double t128 = small <= CUS ? 0.7 * steps + 2.5 : (small <= 2 * CUS ? 1.0 : small / (2.0 * CUS) + 0.5) * (0.9 * steps + 2.5);
+    return t128 < t256;
+}
 
 Plan make_plan(int64_t n, int64_t v, int d, int dtype)
 {
@@ -803,8 +816,6 @@ Plan make_plan(int64_t n, int64_t v, int d, int dtype)
     p.direct = dtype != T_F32 && d % 8 == 0;
     p.n_pad = up(n, 256);
     p.small = n <= 32;
-    p.quarter = up(n, 256) / 256 * (up(v, 256) / 256) <= CUS;      // (4096 x 1000 x 48 fp32: 26 instead of 44 us of tiles)
-    p.sbm = p.quarter && !p.small ? 128 : 256;
     int64_t most = DZ_BYTES / (p.n_pad * 2 * p.parts), packed = WPACK_BYTES / ((int64_t)p.dp * 2 * p.parts) / 256 * 256;
     if (packed < 256) packed = 256;
     if (!p.direct && packed < most) most = packed;
@@ -816,39 +827,45 @@ Plan make_plan(int64_t n, int64_t v, int d, int dtype)
     p.vf = p.vf < up(v, 256) ? p.vf : up(v, 256);
     const int64_t pieces = (v + most - 1) / most;
     p.vc = up((v + pieces - 1) / pieces, 256);
-    p.bm = d > 128 ? 256 : (d > 64 ? 128 : 64);
-    // The products of a piece are cut over k into jobs of about `job` steps (64 deep); the cut with the least estimated time is
-    // taken.  In steps: a job's own cost (its first requests, its results), what the partial sums cost to write and read again,
-    // and for more jobs than the chip holds at once (BM 256: one per CU, else two) their average plus half a long one.
-    const int bn = p.bm == 128 ? 128 : 256;
-    const int64_t tm = (p.dp + p.bm - 1) / p.bm, seg = p.parts == 3 ? 6 : 1;
-    const int64_t tiles_w = tm * ((p.vc + bn - 1) / bn), tiles_x = tm * ((n + bn - 1) / bn);
-    const int64_t steps_w = seg * (up(n, 64) / 64), steps_x = seg * (p.vc / 64);
-    const int64_t slots = p.bm == 256 ? CUS : 2 * CUS;
+    const int64_t steps = (int64_t)(p.parts == 3 ? 6 : 1) * (p.dp / 64);
+    p.quarter_fwd = by_quarters(n, p.vf < v ? p.vf : v, steps);
+    p.quarter_bwd = by_quarters(n, p.vc < v ? p.vc : v, steps);
+    p.sbm = p.quarter_fwd && !p.small ? 128 : 256;
+    // The products of a piece are cut over k into jobs of about `job` steps (64 deep), by tiles of 256 x 256 (one per CU) or
+    // 128 x 128 (two); what has the least estimated time is taken.  In us: a job's steps and its own cost (its first
+    // requests, its results), what the partial sums cost to write and read again, and for more jobs than the chip holds
+    // at once their average plus half a long one.
     double best = 0.0;
-    for (int64_t job = 4;; job += job / 4 + 1) {
-        auto cut = [&](int64_t steps) {
-            const int64_t s = (steps + job - 1) / job;
-            return s < 1 ? (int64_t)1 : (s > 64 ? (int64_t)64 : s);
-        };
-        const int64_t sw = cut(steps_w), sx = cut(steps_x);
-        const double lw = (double)((steps_w + sw - 1) / sw) + JOB_STEPS, lx = (double)((steps_x + sx - 1) / sx) + JOB_STEPS;
-        const double jobs = (double)(tiles_w * sw + tiles_x * sx), all = tiles_w * sw * lw + tiles_x * sx * lx;
-        const double longest = lw > lx ? lw : lx;
-        double t = jobs <= slots ? longest : all / slots + longest / 2;
-        t = t > longest ? t : longest;
-        t += 8.0 * p.dp * (double)(sx * n + (sw > 1 ? sw * p.vc : 0)) / (p.bm == 256 ? 6.4e6 : 3.2e6);
-        if (best == 0.0 || t < best) {
-            best = t;
-            p.split_dw = (int)sw;
-            p.split_dx = (int)sx;
-            p.x_first = lx > lw;
+    for (int bm = 128; bm <= 256; bm *= 2) {
+        const int64_t tm = (p.dp + bm - 1) / bm, seg = p.parts == 3 ? 6 : 1;
+        const int64_t tiles_w = tm * ((p.vc + bm - 1) / bm), tiles_x = tm * ((n + bm - 1) / bm);
+        const int64_t steps_w = seg * (up(n, 64) / 64), steps_x = seg * (p.vc / 64);
+        const int64_t slots = bm == 256 ? CUS : 2 * CUS;
+        const double step = bm == 256 ? STEP_256 : STEP_128;
+        for (int64_t job = 4;; job += job / 4 + 1) {
+            auto cut = [&](int64_t steps) {
+                const int64_t s = (steps + job - 1) / job;
+                return s < 1 ? (int64_t)1 : (s > 64 ? (int64_t)64 : s);
+            };
+            const int64_t sw = cut(steps_w), sx = cut(steps_x);
+            const double lw = (double)((steps_w + sw - 1) / sw) + JOB_STEPS, lx = (double)((steps_x + sx - 1) / sx) + JOB_STEPS;
+            const double jobs = (double)(tiles_w * sw + tiles_x * sx), all = tiles_w * sw * lw + tiles_x * sx * lx;
+            const double longest = lw > lx ? lw : lx;
+            double t = jobs <= slots ? longest : all / slots + longest / 2;
+            t = (t > longest ? t : longest) * step;
+            t += 8.0 * p.dp * (double)(sx * n + (sw > 1 ? sw * p.vc : 0)) / 6.4e6;
+            if (best == 0.0 || t < best) {
+                best = t;
+                p.bm = bm;
+                p.split_dw = (int)sw;
+                p.split_dx = (int)sx;
+                p.x_first = lx > lw;
+            }
+            if (sw == 1 && sx == 1) break;
         }
-        if (sw == 1 && sx == 1) break;
     }
     return p;
 }
-
 
 struct Space {          // hands out 256-byte aligned ranges; with base == NULL only counts
     unsigned char *base;
@@ -923,7 +940,7 @@ void head_of(const Plan &p, const HeadArgs &a, hipStream_t st)
 {
     // (four stages of the small tile: 1 x 32768 x 512 bf16 8.4 us, three 9.6, seven with one workgroup per CU 10.2)
     if (!DZ && p.small) launch_head<Tile<256, 32, 4, 1, false, false, F16, 4>, false, PARTS>(a, st);
-    else if (p.quarter) launch_head<Tile<128, 128, 2, 2, false, false, F16>, DZ, PARTS>(a, st);
+    else if (DZ ? p.quarter_bwd : p.quarter_fwd) launch_head<Tile<128, 128, 2, 2, false, false, F16>, DZ, PARTS>(a, st);
     else launch_head_walk<DuoTile<256, 256, 2, 4, false, false, F16>, DZ, PARTS>(a, st);
 }
 template <bool DZ>
@@ -948,8 +965,7 @@ void launch_products(const Plan &p, ProdArgs w, ProdArgs x, hipStream_t st)
 template <bool F16>
 void products_of(const Plan &p, const ProdArgs &w, const ProdArgs &x, hipStream_t st)
 {
-    if (p.bm == 64) launch_products<Tile<64, 256, 1, 4, true, true, F16>, Tile<64, 256, 1, 4, true, false, F16>>(p, w, x, st);
-    else if (p.bm == 128) launch_products<Tile<128, 128, 2, 2, true, true, F16>, Tile<128, 128, 2, 2, true, false, F16>>(p, w, x, st);
+    if (p.bm == 128) launch_products<Tile<128, 128, 2, 2, true, true, F16>, Tile<128, 128, 2, 2, true, false, F16>>(p, w, x, st);
     else launch_products<DuoTile<256, 256, 2, 4, true, true, F16>, DuoTile<256, 256, 2, 4, true, false, F16>>(p, w, x, st);
 }
 void products(const Plan &p, const ProdArgs &w, const ProdArgs &x, hipStream_t st)
