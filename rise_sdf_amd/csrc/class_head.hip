@@ -44,6 +44,16 @@ __device__ __forceinline__ unsigned short f2bf(float f) { return __builtin_bit_c
 __device__ __forceinline__ unsigned short f2hf(float f) { return __builtin_bit_cast(unsigned short, (_Float16)f); }
 template <bool F16> __device__ __forceinline__ unsigned short to16(float f) { return F16 ? f2hf(f) : f2bf(f); }
 
+// two at once, the first in the low half
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+template <bool F16> __device__ __forceinline__ unsigned to16_two(float a, float b)
+{
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    const f32x2 v = {a, b};
+    return F16 ? __builtin_bit_cast(unsigned, __builtin_convertvector(v, h2)) : __builtin_bit_cast(unsigned, __builtin_convertvector(v, b2));
+}
+
 template <int DT> __device__ __forceinline__ float load1(const void *p, int64_t i)
 {
     if (DT == T_F32) return ((const float *)p)[i];
@@ -78,6 +88,17 @@ __device__ __forceinline__ void split3(float v, unsigned short (&h)[3])
     const float r1 = fin ? v - a : 0.0f;
     h[1] = f2bf(r1);
     h[2] = f2bf(r1 - bf2f(h[1]));
+}
+
+// of two finite numbers (others become NaN)
+__device__ __forceinline__ void split3_two(float a, float b, unsigned *h)
+{
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+        h[k] = to16_two<false>(a, b);
+        a -= __builtin_bit_cast(float, h[k] << 16);
+        b -= __builtin_bit_cast(float, h[k] & 0xffff0000u);
+    }
 }
 
 // (maximum, sum of 2^(. - maximum)) of two sets; a set without a finite element has maximum -inf and a sum of 0 or NaN
@@ -214,8 +235,8 @@ __device__ __forceinline__ void head_tile(const HeadArgs &a, int64_t t, Operand 
     X.lim = (int)(a.n - 1 - n0 < TL::BN - 1 ? a.n - 1 - n0 : TL::BN - 1);
 }
 
-// per row: lse, the weight relative to the largest (0: the row takes part in nothing, whatever its logits are), the label's class
-// relative to the tile's first
+// per row: the weight f relative to the largest (0: the row takes part in nothing, whatever its logits are), lse - log2 |f| (the weight goes
+// into the exponent), the label's class relative to the tile's first
 template <class TL>
 struct RowState {
     float lse[TL::NT], f[TL::NT];
@@ -242,8 +263,8 @@ struct RowState {
 #pragma unroll
         for (int nt = 0; nt < TL::NT; ++nt) {
             const bool live = TL::n_of(nt) < rows && lse[nt] != __builtin_inff();
-            lse[nt] = live ? lse[nt] : __builtin_inff();
             f[nt] = live ? f[nt] / top * (TL::F16 ? F16_DZ : 1.0f) : 0.0f;      // (equal weights: exactly 1)
+            lse[nt] -= __builtin_amdgcn_logf(fabsf(f[nt]));
             label[nt] = f[nt] != 0.0f && a.label != nullptr ? label[nt] - first : -1;
         }
     }
@@ -301,42 +322,44 @@ __device__ __forceinline__ void head_results(const HeadArgs &a, typename TL::Acc
         constexpr bool F16 = TL::F16;
 #pragma unroll
         for (int nt = 0; nt < TL::NT; ++nt) {
-            const int64_t n = n0 + TL::n_of(nt);
             const float lse = rows.lse[nt], f = rows.f[nt];
-            const int label = rows.label[nt];
+            unsigned short *to = a.dz + (n0 + TL::n_of(nt)) * a.ldz + m0;
 #pragma unroll
             for (int b = 0; b < TL::MT / 4; ++b) {
-                const int m = TL::m_of(b);
+                const int m = TL::m_of(b), label = rows.label[nt] - m;
                 float p[16];
 #pragma unroll
                 for (int e = 0; e < 16; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(acc[4 * b + (e >> 2)][nt][e & 3], a.c, -lse));
-                if (label >= m && label < m + 16) {
+                if (f < 0.0f) {
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) p[e] -= m + e == label ? 1.0f : 0.0f;
+                    for (int e = 0; e < 16; ++e) p[e] = -p[e];
                 }
+                if (label >= 0 && label < 16) {
 #pragma unroll
-                for (int e = 0; e < 16; ++e) p[e] *= f;
-                if (f == 0.0f || !whole) {
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) p[e] = f != 0.0f && m + e < left ? p[e] : 0.0f;
+                    for (int e = 0; e < 16; ++e) p[e] -= e == label ? f : 0.0f;
                 }
-                unsigned short o[PARTS][16];
+                if (!whole) {
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    if (PARTS == 3) {
-                        unsigned short h[3];
-                        split3(p[e], h);
+                    for (int e = 0; e < 16; ++e) p[e] = e < left - m ? p[e] : 0.0f;
+                }
+                u32x4 o[PARTS][2];
 #pragma unroll
-                        for (int k = 0; k < PARTS; ++k) o[k][e] = h[k];
-                    } else {
-                        o[0][e] = to16<F16>(p[e]);
-                    }
+                for (int e = 0; e < 16; e += 2) {
+                    unsigned h[PARTS];
+                    if (PARTS == 3) split3_two(p[e], p[e + 1], h);
+                    else h[0] = to16_two<F16>(p[e], p[e + 1]);
+#pragma unroll
+                    for (int k = 0; k < PARTS; ++k) o[k][e >> 3][(e >> 1) & 3] = h[k];
+                }
+                if (f == 0.0f) {
+#pragma unroll
+                    for (int k = 0; k < PARTS; ++k) o[k][0] = o[k][1] = u32x4{0u, 0u, 0u, 0u};
                 }
 #pragma unroll
                 for (int k = 0; k < PARTS; ++k) {
-                    u32x4 *d = (u32x4 *)(a.dz + (k * a.n_pad + n) * a.ldz + m0 + m);
-                    d[0] = ((const u32x4 *)o[k])[0];
-                    d[1] = ((const u32x4 *)o[k])[1];
+                    u32x4 *d = (u32x4 *)(to + k * a.n_pad * a.ldz + m);
+                    d[0] = o[k][0];
+                    d[1] = o[k][1];
                 }
             }
         }
