@@ -724,7 +724,7 @@ int rsdf_embedding_bwd(const int64_t *ids, int64_t n, const void *grad, int64_t 
  *             nothing.  temperature 1.
  *   teacher   ids [n][k], teacher_logits [n][k] (the teacher's top logits): entries with id < 0 are absent whatever their logit
  *             holds; q = softmax of the others / temperature; loss_n = temperature^2 sum_k q_k (log q_k - log softmax(z /
- *             temperature)[ids_k]).  A row without an entry (or with logits of -inf only) takes part in nothing.
+ *             temperature)[ids_k]), temperature in [1e-6, 1e6].  A row without an entry (or with logits of -inf only) takes part in nothing.
  * Rows that take part in nothing have loss 0 and zero gradients and add nothing to dw, whatever x holds there.  A label or
  * listed id outside [0, v) makes its row's loss NaN, adds nothing to the gradients and is counted into *bad_ids (nullable,
  * accumulates).

@@ -1077,7 +1077,7 @@ int rsdf_class_head_fwd(const void *x, const void *w, int64_t n, int64_t v, int 
 {
     const char *bad = bad_head(n, v, d, dtype, k, x, w);
     RSDF_CHECK_ARG(bad == nullptr, bad);
-    RSDF_CHECK_ARG(temperature > 0.0f, "class_head_fwd: temperature must be positive");
+    RSDF_CHECK_ARG(temperature >= 0.999e-6f && temperature <= 1.001e6f, "class_head_fwd: temperature must be in [1e-6, 1e6]");
     RSDF_CHECK_ARG(teacher_logits != nullptr ? (q != nullptr && listed_z != nullptr) : k == 1,
                    "class_head_fwd: a teacher needs q and listed_z, labels need k = 1");
     RSDF_CHECK_ARG(reduction >= 0 && reduction <= 2, "class_head_fwd: reduction must be 0 (none), 1 (mean) or 2 (sum)");

@@ -111,3 +111,15 @@ def test_nodes_load_and_report_errors_as_the_library_does():
     ids, table = torch.zeros(2, dtype=torch.int64), torch.zeros(3, (1 << 16) + 1)
     with pytest.raises((ERR, RuntimeError)):
         n.embedding(ids, table, 1.0, -1, 0)
+
+
+def test_temperatures_out_of_range():
+    """T^2 and 1 / T have to stay far inside fp32."""
+    x, w = torch.zeros(4, 8), torch.zeros(10, 8)
+    ids, lg = torch.zeros(4, 3, dtype=torch.int64), torch.zeros(4, 3)
+    for t in (1e-7, 2e6, 1e30):
+        with pytest.raises(ERR, match="temperature"):
+            linear_distillation(x, w, ids, lg, temperature=t)
+    l = _lib.lib()
+    for t in (0.0, 1e-7, 2e6, float("nan")):
+        assert l.rsdf_class_head_fwd(None, None, 4, 8, 8, 0, None, None, 1, -100, t, 0, None, None, None, None, None, None, None, 1 << 30, None) != 0

@@ -269,3 +269,43 @@ def test_nothing_is_written_around_the_results(dev, n, v, d, dtype):
         assert bool((t[size:] == 77).all())
     assert torch.equal(pair["loss"][1][0], a[0]) and torch.equal(pair["dx"][1], a[1]) and torch.equal(pair["dw"][1], a[2])
     assert torch.equal(pair["out"][1], w[y])
+
+
+def test_other_modes_of_torch(dev):
+    """Inference mode, autocast, checkpointing, accumulated .grad; a teacher's logits of any floating type, which take no gradient."""
+    from torch.utils.checkpoint import checkpoint
+    x, w, y = head_case(dev, 130, 300, 48, F32, seed=100)
+    ids, table, _ = lookup_case(dev, 130, 90, 48, F32, seed=101)
+    tid, tl = teacher(dev, 130, 300, 6, seed=102)
+    loss, dx, dw = check_head(x, w, y)
+    with torch.inference_mode():
+        assert torch.equal(linear_cross_entropy(x, w, y), loss)
+        assert torch.equal(ops.embedding(ids, table), table[ids])
+    with torch.autocast("cuda", dtype=BF16):
+        assert torch.equal(linear_cross_entropy(x, w, y), loss)
+    xr, wr = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    for _ in range(2):
+        checkpoint(lambda a, b: linear_cross_entropy(a, b, y), xr, wr, use_reentrant=False).backward()
+    assert torch.equal(xr.grad, dx + dx) and torch.equal(wr.grad, dw + dw)
+    half = tl.to(BF16)
+    a = linear_distillation(x, w, tid, half, temperature=2.0)
+    assert torch.equal(a, linear_distillation(x, w, tid, half.double(), temperature=2.0))
+    soft = tl.clone().requires_grad_(True)
+    assert not linear_distillation(x, w, tid, soft).requires_grad
+    both = linear_distillation(x.clone().requires_grad_(True), w, tid.t().contiguous().t(), soft)
+    both.backward()
+    assert soft.grad is None
+
+
+def test_temperatures_at_the_ends(dev):
+    """1 / T of the logits' spread: at 1e-6 the teacher is its largest logit, at 1e6 uniform; what is left of the loss (T^2 times a divergence
+    near 1 / T^2) is rounding, so only the gradient, T times a difference of probabilities, is compared: within T e."""
+    x, w, _ = head_case(dev, 40, 200, 32, F32, seed=103)
+    tid, tl = teacher(dev, 40, 200, 5, seed=104, missing=0.0)
+    for t in (1e-6, 1e6):
+        xr = x.clone().requires_grad_(True)
+        loss = linear_distillation(xr, w, tid, tl, temperature=t, reduction="sum")
+        (dx,) = torch.autograd.grad(loss, xr)
+        want = ref.head(x, w, tid, tl, -100, t, "sum", torch.ones((), device=dev))
+        assert not bool(torch.isnan(loss)) and bool(torch.isfinite(dx).all())
+        ref.assert_within("dx", dx, want["dx"], want["e_dx"])
