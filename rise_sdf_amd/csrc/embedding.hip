@@ -5,7 +5,7 @@
 //
 // Both are bound by memory: the lookup reads each row that occurs and writes N rows, the gradient reads N rows and writes V.
 // Products and sums are fp32, one rounding to the table's type at the end.  262144 rows of 65536 x 256 bf16: lookup 28 us (6 TB/s:
-// the popular rows come from the caches), gradient 79 (sort 34, sums 28, joins 17).
+// the popular rows come from the caches), gradient 76 (sort 33, sums 33, joins 10).
 //
 // The gradient sorts the positions by id (a stable radix sort) and sums the rows of one id in
 // order: no float atomics, the same bits every time.  The sorted list is cut into chunks of equal LENGTH, so an id that takes
@@ -215,51 +215,108 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_scatter_kernel(const int64_
     }
 }
 
-// ---- few positions: no list -----------------------------------------------------------------------------------------------------
-// One wave per row of the table walks all ids, 64 at a time, and adds up its positions in order: one launch, no workspace.
+// ---- few positions: no sort -----------------------------------------------------------------------------------------------------
+// One launch, no workspace: a wave per row of the table looks through all ids, 64 at a time, and lists the first LIGHT positions of its
+// row.  Groups of lanes (as many as a row of vectors needs) take every so-manieth position, and their sums are added in order.  A row
+// with more positions, the one id of a whole batch for instance, is listed again and added up by all four waves.
+// Against sorting (four or five launches; both in us of kernels): 256 positions of 100 x 48 fp32 4.1 and 13.1, 1024 of 4000 x 48 7.1 and 19,
+// 512 of 16000 x 64 10.6 and 20, one id for 512 rows of 512 fp32 15.2 and 15.2; but one id for 2048 such rows 73 and 22, 100 of 60000
+// x 48 30 and 19: so up to FEW positions of FEW_ROWS rows.
+constexpr int LIGHT = 64, FEW = 1024;
+constexpr int64_t FEW_ROWS = 16384;
 template <int DT, int VW>
 __global__ void __launch_bounds__(256) few_kernel(const int64_t *__restrict__ ids, int n, const void *__restrict__ g, int64_t v, int d, int per_row,
-                                                  float scale, int64_t padding, void *__restrict__ out)
+                                                  int lanes, float scale, int64_t padding, void *__restrict__ out)
 {
     using E = Elem<DT>;
     using T = typename E::type;
     using V = Vec<T, VW>;
-    const int lane = threadIdx.x & 63;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= v) return;
-    for (int c = lane; c - lane < per_row; c += 64) {
-        float acc[VW];
-        const int col = element_of<V>(c < per_row ? c : 0, d);
+    constexpr int U = 8;                                 // rows on their way at once
+    __shared__ unsigned short list[FEW];                 // LIGHT of each wave; all of one row
+    __shared__ int counts[4];
+    __shared__ float sums[256 * VW];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int64_t first = (int64_t)blockIdx.x * 4;
+    const unsigned long long below = (1ull << lane) - 1;
+
+    // positions of a row into a list of at most `most`; their number
+    auto look = [&](int64_t row, unsigned short *to, int most) {
+        int count = 0;
+        for (int i0 = 0; i0 < n; i0 += 64 * U) {
+            bool mine[U];
 #pragma unroll
-        for (int k = 0; k < VW; ++k) acc[k] = 0.0f;
-        for (int i0 = 0; i0 < n; i0 += 64) {
-            const bool mine = i0 + lane < n && ids[i0 + lane] == row && row != padding;
-            unsigned long long m = __ballot(mine);
-            while (m != 0) {
-                constexpr int U = 8;                     // rows on their way at once
-                V x[U];
-                int here = 0;
+            for (int u = 0; u < U; ++u) {
+                const int i = i0 + u * 64 + lane;
+                mine[u] = ids[i < n ? i : 0] == row && i < n;
+            }
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    if (m == 0) continue;
-                    const int at = i0 + __ffsll((long long)m) - 1;
-                    m &= m - 1;
-                    here = u + 1;
-                    x[u] = load_at<V>((const T *)g, (int64_t)at * d + col);
-                }
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    if (u >= here) continue;
-#pragma unroll
-                    for (int k = 0; k < VW; ++k) acc[k] += E::get(x[u].v[k]);
-                }
+            for (int u = 0; u < U; ++u) {
+                const unsigned long long m = __ballot(mine[u]);
+                const int at = count + __popcll(m & below);
+                if (mine[u] && at < most) to[at] = (unsigned short)(i0 + u * 64 + lane);
+                count += __popcll(m);
             }
         }
-        if (c < per_row) {
-            V o;
+        return count;
+    };
+    // vector c of the positions k, k + step, ... of a list
+    auto add = [&](float (&acc)[VW], const unsigned short *from, int count, int k, int step, int c) {
+        const int col = element_of<V>(c, d);
 #pragma unroll
-            for (int k = 0; k < VW; ++k) o.v[k] = E::put(acc[k] * scale);
-            store_at<false>((T *)out, row * d + col, o);
+        for (int e = 0; e < VW; ++e) acc[e] = 0.0f;
+        for (; k < count; k += step * U) {
+            V x[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) x[u] = load_at<V>((const T *)g, (int64_t)from[k + u * step < count ? k + u * step : k] * d + col);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int e = 0; e < VW; ++e) acc[e] += k + u * step < count ? E::get(x[u].v[e]) : 0.0f;
+        }
+    };
+    auto put = [&](const float (&acc)[VW], int64_t row, int c) {
+        V o;
+#pragma unroll
+        for (int e = 0; e < VW; ++e) o.v[e] = E::put(acc[e] * scale);
+        store_at<false>((T *)out, row * d + element_of<V>(c, d), o);
+    };
+
+    const int64_t row = first + w;
+    const int count = row < v && row != padding ? look(row, list + w * LIGHT, LIGHT) : 0;
+    if (lane == 0) counts[w] = count;
+    __builtin_amdgcn_wave_barrier();
+    if (row < v && count <= LIGHT) {
+        const int in_wave = lanes < 64 ? lanes : 64, groups = 64 / in_wave, k = lane / in_wave;
+        for (int c0 = 0; c0 < per_row; c0 += in_wave) {
+            const int c = c0 + lane % in_wave;
+            float acc[VW];
+            add(acc, list + w * LIGHT, c < per_row ? count : 0, k, groups, c < per_row ? c : 0);
+            for (int o = 32; o >= in_wave; o >>= 1)
+#pragma unroll
+                for (int e = 0; e < VW; ++e) acc[e] += __shfl_xor(acc[e], o, 64);
+            if (k == 0 && c < per_row) put(acc, row, c);
+        }
+    }
+    __syncthreads();
+    for (int heavy = 0; heavy < 4; ++heavy) {
+        if (counts[heavy] <= LIGHT) continue;
+        if (w == heavy) look(row, list, FEW);
+        __syncthreads();
+        const int groups = 256 / lanes, k = threadIdx.x / lanes;
+        for (int c0 = 0; c0 < per_row; c0 += lanes) {
+            const int c = c0 + threadIdx.x % lanes;
+            float acc[VW];
+            add(acc, list, c < per_row ? counts[heavy] : 0, k, groups, c < per_row ? c : 0);
+#pragma unroll
+            for (int e = 0; e < VW; ++e) sums[e * 256 + threadIdx.x] = acc[e];
+            __syncthreads();
+            if (k == 0 && c < per_row) {
+                for (int j = 1; j < groups; ++j)
+#pragma unroll
+                    for (int e = 0; e < VW; ++e) acc[e] += sums[e * 256 + j * lanes + threadIdx.x];
+                put(acc, first + heavy, c);
+            }
+            __syncthreads();
         }
     }
 }
@@ -446,10 +503,10 @@ Sorting sorting(int64_t n, int64_t v)
     return s;
 }
 
-int chunk_of(int64_t n) { const int64_t c = n / 8192; return (int)(c < 8 ? 8 : (c > 64 ? 64 : c)); }
+// (sums and joins of 262144 x 256 bf16: chunks of 8 83 us, of 32 46, of 64 43; of 10000 x 250 fp32: 15, 18, 28; of 100000 x 64: 20, 21, 31)
+int chunk_of(int64_t n) { const int64_t c = n / 4096; return (int)(c < 8 ? 8 : (c > 64 ? 64 : c)); }
 
-// Walking all ids per row of the table instead of sorting them: n / 64 steps for each of v waves, and every addition of a row in turn
-bool use_few(int64_t n, int64_t v) { return n > 0 && n <= 512 && n * v <= (1 << 23); }
+bool use_few(int64_t n, int64_t v) { return n > 0 && n <= FEW && v <= FEW_ROWS; }
 
 struct Space { unsigned *keys[2], *pos[2], *counts; unsigned char *goes_on; float *part; int64_t bytes; };
 Space space(void *ws, int64_t n, int64_t v, int d)
@@ -547,7 +604,10 @@ int rsdf_embedding_bwd(const int64_t *ids, int64_t n, const void *grad, int64_t 
     const int bytes = vector_bytes(d, dtype), size = dtype == T_F32 ? 4 : 2;
     const int per_row = (d * size + bytes - 1) / bytes;
     if (use_few(n, v)) {
-#define CALL(DT, VW) few_kernel<DT, VW><<<(unsigned)((v + 3) / 4), 256, 0, st>>>(ids, (int)n, grad, v, d, per_row, scale, padding_id, d_table)
+        int lanes = 1;
+        while (lanes < per_row && lanes < 256) lanes *= 2;
+#define CALL(DT, VW) \
+    few_kernel<DT, VW><<<(unsigned)((v + 3) / 4), 256, 0, st>>>(ids, (int)n, grad, v, d, per_row, lanes, scale, padding_id, d_table)
         RSDF_EMBEDDING_DISPATCH(dtype, bytes, CALL);
 #undef CALL
         RSDF_RETURN_LAUNCH();

@@ -309,3 +309,25 @@ def test_temperatures_at_the_ends(dev):
         want = ref.head(x, w, tid, tl, -100, t, "sum", torch.ones((), device=dev))
         assert not bool(torch.isnan(loss)) and bool(torch.isfinite(dx).all())
         ref.assert_within("dx", dx, want["dx"], want["e_dx"])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,v,d", [(65, 4, 48), (64, 1, 5), (1024, 9, 48), (1024, 16384, 20), (1024, 5, 2100), (700, 3, 512), (1023, 2, 1),
+                                   (1025, 5, 48), (512, 16385, 8)])
+def test_lookup_of_one_batch_with_few_ids(dev, n, v, d, dtype):
+    """A batch whose positions name one id, two ids, or an id and the padding: as one view's rays do.  Also around the sizes from
+    which the positions are sorted."""
+    ids, table, grad = lookup_case(dev, n, v, d, dtype, "same", seed=n)
+    check_lookup(ids, table, grad, 1.0, None)
+    ids[::3] = 0
+    check_lookup(ids, table, grad, 0.5, None)
+    if v > 1:
+        check_lookup(ids, table, grad, 0.5, 0)
+    ids[5:60] = torch.randint(0, v, (55,), device=dev, generator=gen(dev, 110))
+    ids[7] = v                                              # outside: no part in the gradient
+    t = table.clone().requires_grad_(True)
+    (dt,) = torch.autograd.grad(ops.embedding(ids, t), t, grad)
+    _, _, want, bound = ref.embedding(ids, table, 1.0, None, grad)
+    ref.assert_within("d_table", dt, want, bound)
+    with pytest.raises(_lib.RiseSdfHipError, match="outside"):
+        _lib.poll_status(dev)
