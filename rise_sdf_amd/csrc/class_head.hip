@@ -9,7 +9,9 @@
 // Cross entropy is the distillation of one entry with q = 1 and T = 1, so one set of kernels serves both.
 //
 // Forward: the tiles of z never leave the registers: each writes its rows' maximum and sum of exponentials, and one wave per row
-// joins them and takes the logits of the K listed classes as K dot products.
+// joins them and takes the logits of the K listed classes as K dot products.  The first listed class (the label) is left out of
+// the tiles' sums and joined from its dot product: with R the sum over the others, lse - z_y = log(1 + R exp(-z_y)) and
+// 1 - p_y = 1 / (1 + exp(z_y) / R) keep all their digits where the head is sure of itself, and both uses of z_y see one rounding.
 // Backward, in pieces of the classes: the tiles are computed again and leave as 16-bit dz [rows][piece]; two products read it
 // (dx over the piece, dw of the piece).  A piece is at most DZ_BYTES: it is still in the last-level cache when it is read
 // (products at V = 131072: 1005 us; with 64 MB pieces, twice as many launches, 1267, with 256 MB 1273).
@@ -217,9 +219,10 @@ struct HeadArgs {
     float2 *stats;               // [class tile][n]: maximum and sum of 2^(c z - maximum)
     int64_t tile0;               // first class tile of the piece
     // dz
-    const float *lse;            // [n] in powers of two; +inf: a row that takes part in nothing
+    const float *lse;            // [n] in powers of two; +inf: a row that takes part in nothing; [n] 1 - p of the first listed class
     const float *weight, *top;   // [n], [1]
-    const int64_t *label;        // [n] or NULL
+    const int64_t *label;        // first listed class of a row, label_step apart (dz: labels, or NULL)
+    int64_t label_step;
     int64_t v0;
     unsigned short *dz;          // [parts][n_pad][ldz]
     int64_t n_pad, ldz;
@@ -275,13 +278,39 @@ struct RowState {
     }
 };
 
+// what a tile needs of its rows: the state above for dz, for statistics the class that is left out, relative to the head's first
+// (one that is not there: -1)
+template <class TL, bool DZ>
+struct TileRows : RowState<TL> {};
+template <class TL>
+struct TileRows<TL, false> {
+    int label[TL::NT];
+    int2 raw[TL::NT];
+    __device__ __forceinline__ void request(const HeadArgs &a, int64_t n0)
+    {
+#pragma unroll
+        for (int nt = 0; nt < TL::NT; ++nt) {
+            const int64_t n = n0 + TL::n_of(nt);
+            raw[nt] = *(const int2 *)(a.label + (n < a.n ? n : a.n - 1) * a.label_step);
+        }
+    }
+    __device__ __forceinline__ void load(const HeadArgs &, int64_t, int64_t)
+    {
+#pragma unroll
+        for (int nt = 0; nt < TL::NT; ++nt) {
+            label[nt] = raw[nt].y == 0 ? raw[nt].x : -1;
+            asm volatile("" ::"v"(label[nt]));       // (here, as above)
+        }
+    }
+};
+
 template <class TL, bool DZ, int PARTS>
-__device__ __forceinline__ void head_results(const HeadArgs &a, typename TL::Acc &acc, const RowState<TL> &rows, int64_t m0, int64_t n0,
+__device__ __forceinline__ void head_results(const HeadArgs &a, typename TL::Acc &acc, const TileRows<TL, DZ> &rows, int64_t m0, int64_t n0,
                                              float2 *part /* [WM][BN], LDS */)
 {
     const bool whole = a.vc - m0 >= TL::BM;     // else the last classes of the tile are not there
     const int left = whole ? TL::BM : (int)(a.vc - m0);      // (0 or less: a tile of zeros)
-    if (!DZ) {
+    if constexpr (!DZ) {
         const int lane = my_lane(), wm = my_wave() / TL::WN;
         if (!whole) {
 #pragma unroll
@@ -293,8 +322,18 @@ __device__ __forceinline__ void head_results(const HeadArgs &a, typename TL::Acc
                     for (int r = 0; r < 4; ++r) acc[mt][nt][r] = m + r < left ? acc[mt][nt][r] : -__builtin_inff();
             }
         }
+        const int wave_m = (int)(a.v0 + m0) + wm * TL::TM;
 #pragma unroll
         for (int nt = 0; nt < TL::NT; ++nt) {
+            const int label = rows.label[nt] - wave_m;
+            if (label >= 0 && label < TL::TM) {
+#pragma unroll
+                for (int b = 0; b < TL::MT / 4; ++b) {
+                    const int l = label - (TL::m_of(b) - wm * TL::TM);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) acc[4 * b + (e >> 2)][nt][e & 3] = e == l ? -__builtin_inff() : acc[4 * b + (e >> 2)][nt][e & 3];
+                }
+            }
             // (c > 0: the maximum of z is that of c z; one fma, one exponential and one sum per logit)
             float mx = -__builtin_inff();
 #pragma unroll
@@ -340,8 +379,9 @@ __device__ __forceinline__ void head_results(const HeadArgs &a, typename TL::Acc
                     for (int e = 0; e < 16; ++e) p[e] = -p[e];
                 }
                 if (label >= 0 && label < 16) {
+                    const float miss = a.lse[a.n + n0 + TL::n_of(nt)];
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) p[e] -= e == label ? f : 0.0f;
+                    for (int e = 0; e < 16; ++e) p[e] = e == label ? -miss * f : p[e];
                 }
                 if (!whole) {
 #pragma unroll
@@ -394,9 +434,10 @@ __global__ void __launch_bounds__(TL::THREADS, TL::OCCUPANCY) head_kernel(HeadAr
     clear<TL>(acc);
     const int64_t ksteps = a.depth / TL::KD;
     const bool there = m0 < a.vc && n0 < a.n;
+    TileRows<TL, DZ> rows;
+    if constexpr (!DZ) rows.request(a, n0);
     TL::run(acc, W, X, a.nseg, ksteps, 0, there ? a.nseg * ksteps : 0, lds);
-    RowState<TL> rows;
-    if (DZ) rows.load(a, m0, n0);
+    rows.load(a, m0, n0);
     head_results<TL, DZ, PARTS>(a, acc, rows, m0, n0, (float2 *)lds);
 }
 
@@ -424,9 +465,10 @@ __global__ void __launch_bounds__(TL::THREADS, TL::OCCUPANCY) head_walk_kernel(H
     for (bool later = false;; later = true) {
         typename TL::Acc acc;
         clear<TL>(acc);
+        TileRows<TL, DZ> rows;
+        if constexpr (!DZ) rows.request(a, n0);
         pipe.template finish<STORES>(acc, later);
-        RowState<TL> rows;
-        if (DZ) rows.load(a, m0, n0);
+        rows.load(a, m0, n0);
         const int64_t m = m0, n = n0;
         t += stride;
         if (t < end) {
@@ -449,7 +491,7 @@ struct RowArgs {
     const float *logits;         // [n][k], NULL: cross entropy (k = 1)
     int64_t ignore;              // cross entropy: the label that is left out; distillation leaves out every id < 0
     float temperature;
-    float *loss, *lse, *q, *zt;  // [n], [n], [n][k] (NULL: cross entropy), [n][k] (NULL likewise)
+    float *loss, *lse, *q, *zt;  // [n], [2][n], [n][k] (NULL: cross entropy), [n][k] (NULL likewise)
     int *status;                 // counts ids outside [0, v); may be NULL
 };
 
@@ -497,6 +539,25 @@ __device__ __forceinline__ float dots(const void *x, const void *w, int64_t xo, 
     return s[0];
 }
 
+// one dot product by one wave
+template <int DT, int BYTES>
+__device__ __forceinline__ float dot(const void *x, const void *w, int64_t xo, int64_t wo, int d)
+{
+    constexpr int E = BYTES / (DT == T_F32 ? 4 : 2);
+    using V = typename Words<BYTES>::type;
+    const int lane = threadIdx.x & 63;
+    float s = 0.0f;
+    int i = lane * E;
+    for (; i + E <= d; i += 64 * E) {
+        const V a = load_at<V, DT>(x, xo + i), b = load_at<V, DT>(w, wo + i);
+#pragma unroll
+        for (int e = 0; e < E; ++e) s = fmaf(load1<DT>(&a, e), load1<DT>(&b, e), s);
+    }
+    i = d / E * E + lane;
+    if (E > 1 && i < d) s = fmaf(load1<DT>(x, xo + i), load1<DT>(w, wo + i), s);
+    return wave_sum(s);
+}
+
 // LR rows per workgroup (4; 1 where a teacher's rows are few).  The tiles' statistics are read with rows running
 // fastest, then each wave takes whole rows (1 row: its waves share the listed classes).
 template <int DT, int BYTES, int LR>
@@ -522,18 +583,24 @@ __global__ void __launch_bounds__(256) rows_kernel(RowArgs a)
     for (int rr = LR == 1 ? 0 : wave; rr < LR; rr += 4) {
         const int64_t r = r0 + rr;
         if (r >= a.n) return;                       // (LR 1: r0 < n)
-        const float lse = st[rr].x + __builtin_amdgcn_logf(st[rr].y);     // v_log_f32: base 2
+        const float c = LOG2E * inv_t;
+        const int64_t first = a.ids[r * a.k];
+        // lse = ref + over in powers of two, kept apart: with a first class, over = log(1 + what is smaller, it or the others)
+        const bool pivot = first >= 0 && first < a.v && (a.logits != nullptr || first != a.ignore);
+        const float zp = pivot ? dot<DT, BYTES>(a.x, a.w, r * a.d, first * a.d, a.d) : 0.0f;
+        const float rest = st[rr].x + __builtin_amdgcn_logf(st[rr].y);    // v_log_f32: base 2
+        const float u = zp * c - rest, near = __builtin_amdgcn_exp2f(-fabsf(u));
+        const float ref = pivot ? fmaxf(zp * c, rest) : st[rr].x;
+        const float over = pivot ? log1pf(near) * LOG2E : __builtin_amdgcn_logf(st[rr].y);
+        const float miss = pivot ? 1.0f / (1.0f + __builtin_amdgcn_exp2f(u)) : 1.0f;
+        float lse = ref + over;
+        if (!(fabsf(lse) < __builtin_inff())) lse = __builtin_nanf("");   // (+inf means something else)
         float loss = 0.0f;
         bool alive = false, bad = false;
         if (a.logits == nullptr) {
-            const int64_t id = a.ids[r];
-            bad = id != a.ignore && (id < 0 || id >= a.v);
-            alive = id != a.ignore && !bad;
-            if (alive) {
-                float s = 0.0f;
-                for (int i = lane; i < a.d; i += 64) s = fmaf(load1<DT>(a.x, r * a.d + i), load1<DT>(a.w, id * a.d + i), s);
-                loss = lse * LN2 - wave_sum(s);
-            }
+            bad = first != a.ignore && !pivot;
+            alive = pivot;
+            if (alive) loss = ((ref - zp * c) + over) * LN2 + (lse - lse);
         } else {
             const int64_t *ids = a.ids + r * a.k;
             const float *lg = a.logits + r * a.k;
@@ -554,7 +621,7 @@ __global__ void __launch_bounds__(256) rows_kernel(RowArgs a)
                 for (int k = lane; k < a.k; k += 64)
                     if (ids[k] >= 0) sum += expf((lg[k] - tm) * inv_t);   // (the difference first: logits at the type's ends)
             sum = wave_sum(sum);
-            const float lse_e = lse * LN2, ls = logf(sum);
+            const float ls = logf(sum);
             for (int k0 = LR == 1 ? wave * G : 0; k0 < a.k; k0 += LR == 1 ? 4 * G : G) {
                 int64_t wo[G];
 #pragma unroll
@@ -567,9 +634,10 @@ __global__ void __launch_bounds__(256) rows_kernel(RowArgs a)
                 if (k < a.k && (lane & 7) == 0) {
                     float qk = 0.0f;
                     if (alive && ids[k] >= 0) {
+                        if (ids[k] == first) z = zp;
                         const float lq = (lg[k] - tm) * inv_t - ls;
                         qk = expf(lq);
-                        if (!(qk == 0.0f)) loss += qk * (lq - z * inv_t + lse_e);
+                        if (!(qk == 0.0f)) loss += qk * (lq + ((ref - z * c) + over) * LN2) + (lse - lse);
                     } else {
                         z = 0.0f;
                     }
@@ -591,6 +659,7 @@ __global__ void __launch_bounds__(256) rows_kernel(RowArgs a)
             if (bad && a.status != nullptr) atomicAdd(a.status, 1);
             a.loss[r] = loss;
             a.lse[r] = alive ? lse : __builtin_inff();
+            a.lse[a.n + r] = miss;
         }
     }
 }
@@ -619,7 +688,8 @@ __global__ void __launch_bounds__(1024) sum_kernel(const float *__restrict__ los
     }
 }
 
-// The listed classes' entries of dz: p - (sum of the q of that class in this row); a class listed twice is written twice alike.
+// The listed classes' entries of dz: p - (sum of the q of that class in this row); a class listed twice is written twice alike.  The first
+// class of a row that is sure of it: (1 - q) - (1 - p).
 // One wave per row, its entries 64 at a time in the lanes.
 template <bool F16, int PARTS>
 __global__ void __launch_bounds__(256) listed_kernel(const int64_t *__restrict__ ids, const float *__restrict__ q,
@@ -630,7 +700,8 @@ __global__ void __launch_bounds__(256) listed_kernel(const int64_t *__restrict__
     const int lane = threadIdx.x & 63;
     const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (r >= n) return;
-    const float l = lse[r];
+    const float l = lse[r], miss = lse[n + r];
+    const int64_t first = ids[r * k];
     if (l == __builtin_inff()) return;
     const float f = weight[r] / top[0] * (F16 ? F16_DZ : 1.0f);
     for (int k0 = 0; k0 < k; k0 += 64) {
@@ -647,7 +718,8 @@ __global__ void __launch_bounds__(256) listed_kernel(const int64_t *__restrict__
             }
         }
         if (id < v0 || id >= v0 + vc || s == 0.0f) continue;
-        const float p = f != 0.0f ? (__builtin_amdgcn_exp2f(zt[r * k + i] * c - l) - s) * f : 0.0f;
+        const float pq = id == first && miss < 0.5f ? (1.0f - s) - miss : __builtin_amdgcn_exp2f(zt[r * k + i] * c - l) - s;
+        const float p = f != 0.0f ? pq * f : 0.0f;
         unsigned short h[3];
         if (PARTS == 3) split3(p, h);
         else h[0] = to16<F16>(p);
@@ -1106,6 +1178,8 @@ int rsdf_class_head_fwd(const void *x, const void *w, int64_t n, int64_t v, int 
         a.c = LOG2E / temperature;
         a.stats = f.stats;
         a.tile0 = v0 / p.sbm;
+        a.v0 = v0;
+        a.label = ids; a.label_step = k;
         head<false>(p, a, st);
     }
     RowArgs r = {x, w, n, v, d, k, f.stats, (v + p.sbm - 1) / p.sbm, ids, teacher_logits, ignore_id, temperature,
@@ -1156,7 +1230,7 @@ int rsdf_class_head_bwd(const void *x, const void *w, int64_t n, int64_t v, int 
         a.c = LOG2E / temperature;
         a.lse = lse;
         a.weight = b.weight; a.top = b.top;
-        a.label = q == nullptr ? ids : nullptr;
+        a.label = q == nullptr ? ids : nullptr; a.label_step = 1;
         a.v0 = v0;
         a.dz = b.dz;
         head<true>(p, a, st);

@@ -141,13 +141,13 @@ struct ClassHead : torch::autograd::Function<ClassHead> {
         if (bytes < 0) check(1, "class_head_workspace_bytes");
         const Tensor ws = bytes_on(bytes, x);
         const auto f32 = x.options().dtype(at::kFloat).requires_grad(false);
-        // lse [n], count [1], and for a teacher q, listed logits [n, k]: one allocation, kept for the backward
-        const Tensor keep = at::empty({n + 1 + (teacher ? 2 * n * k : 0)}, f32);
+        // lse [2, n], count [1], and for a teacher q, listed logits [n, k]: one allocation, kept for the backward
+        const Tensor keep = at::empty({2 * n + 1 + (teacher ? 2 * n * k : 0)}, f32);
         Tensor loss = reduction == 0 ? at::empty({n}, f32) : at::empty({}, f32);
-        float *a = address<float>(keep), *q = teacher ? a + n + 1 : nullptr;
+        float *a = address<float>(keep), *q = teacher ? a + 2 * n + 1 : nullptr;
         check(E.class_head_fwd(address<const void>(x), address<const void>(w), n, v, (int)d, dtype_id(x), address<const int64_t>(ids),
                                teacher ? address<const float>(*logits) : nullptr, (int)k, ignore, (float)temperature, (int)reduction,
-                               address<float>(loss), a, a + n, q, teacher ? q + n * k : nullptr, (int32_t *)bad_ids, address<void>(ws), bytes,
+                               address<float>(loss), a, a + 2 * n, q, teacher ? q + n * k : nullptr, (int32_t *)bad_ids, address<void>(ws), bytes,
                                stream_of(x)),
               "class_head_fwd");
         ctx->save_for_backward({x, w, ids, keep});
@@ -174,10 +174,10 @@ struct ClassHead : torch::autograd::Function<ClassHead> {
         if (need_w) out[1] = at::empty_like(w);
         const int64_t bytes = E.class_head_workspace_bytes(n, v, (int)d, dtype_id(x), (need_x ? 1 : 0) + (need_w ? 2 : 0));
         const Tensor ws = bytes_on(bytes, x);
-        float *a = address<float>(keep), *q = teacher ? a + n + 1 : nullptr;
+        float *a = address<float>(keep), *q = teacher ? a + 2 * n + 1 : nullptr;
         check(E.class_head_bwd(address<const void>(x), address<const void>(w), n, v, (int)d, dtype_id(x), address<const int64_t>(ids), q,
                                teacher ? q + n * k : nullptr, (int)k, (float)ctx->saved_data["temperature"].toDouble(), a,
-                               reduction == 1 ? a + n : nullptr, address<const float>(g), reduction == 0, address<void>(out[0]),
+                               reduction == 1 ? a + 2 * n : nullptr, address<const float>(g), reduction == 0, address<void>(out[0]),
                                address<void>(out[1]), address<void>(ws), bytes, stream_of(x)),
               "class_head_bwd");
         return once(std::move(out), "the losses of a linear head");

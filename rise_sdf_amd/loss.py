@@ -180,7 +180,8 @@ def linear_distillation(x, weight, teacher_ids, teacher_logits, *, temperature=1
     Per row: ``T^2 * sum_k q_k (log q_k - log_softmax(x @ weight.T / T)[ids_k])`` with ``q = softmax(teacher_logits / T)`` over
     the listed classes: the divergence from the teacher's renormalised top classes.  ``x`` [..., D], ``weight`` [V, D] of one
     type, ``teacher_ids`` [..., K] integers (negative: no entry, whatever its logit holds; a class may be listed twice),
-    ``teacher_logits`` [..., K] (any floating type, no gradient), ``temperature`` between 1e-6 and 1e6.  Rows without an entry take part in nothing.  ``reduction``: "none" -> [...],
+    ``teacher_logits`` [..., K] (any floating type, no gradient), ``temperature`` between 1e-6 and 1e6.  Where the head is sure of one class, the loss keeps its digits
+    if that class is the first of the list (order a teacher's logits from the largest down).  Rows without an entry take part in nothing.  ``reduction``: "none" -> [...],
     "mean" over the rows with an entry (0 if there are none), "sum"; fp32.  Differentiable w.r.t. ``x`` and ``weight`` (once).
     A listed class >= V makes its row NaN, takes no part in the gradients and is reported by
     ``rise_sdf_amd.check_status()``."""

@@ -243,7 +243,7 @@ def test_nothing_is_written_around_the_results(dev, n, v, d, dtype):
     x, w, y = head_case(dev, n, v, d, dtype, seed=90)
     a = check_head(x, w, y)
     pair = {}
-    for name, shape, t in (("loss", (1,), F32), ("lse", (n,), F32), ("count", (1,), F32), ("dx", (n, d), dtype), ("dw", (v, d), dtype),
+    for name, shape, t in (("loss", (1,), F32), ("lse", (2, n), F32), ("count", (1,), F32), ("dx", (n, d), dtype), ("dw", (v, d), dtype),
                            ("out", (n, d), dtype), ("dt", (v, d), dtype)):
         pair[name] = margin(dev, shape, t, 7.0)
     p = {k: t[1].data_ptr() for k, t in pair.items()}
@@ -331,3 +331,40 @@ def test_lookup_of_one_batch_with_few_ids(dev, n, v, d, dtype):
     ref.assert_within("d_table", dt, want, bound)
     with pytest.raises(_lib.RiseSdfHipError, match="outside"):
         _lib.poll_status(dev)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,v,d", [(2, 183, 80), (3, 1000, 64), (40, 300, 48), (33, 5000, 200), (300, 70000, 64)])
+def test_sure_rows_keep_their_digits(dev, n, v, d, dtype):
+    """Features along their own class: logits of 24 to 30, probabilities within 1e-3 to 1e-11 of 1.  The loss and the label's entry of dz are as small,
+    and have to be right relative to themselves: with R the sum over the other classes, relative to the label, the loss is log(1 + R) and
+    1 - p = R / (1 + R); R's relative error is that of the differences of logits, 2 ez, and of its sum, (300 + V / 8192) e."""
+    g = gen(dev, 120)
+    w = (torch.randn(v, d, device=dev, generator=g) * (3.0 / d ** 0.5)).to(dtype)
+    y = torch.randint(0, v, (n,), device=dev, generator=g)
+    own = w[y].float()
+    x = (own * ((24.0 + 6.0 * torch.rand(n, 1, device=dev, generator=g)) / own.square().sum(1, keepdim=True))).to(dtype)
+    z = x.double() @ w.double().t()
+    mag = x.double().abs() @ w.double().abs().t()
+    rest = torch.exp(z - z.gather(1, y[:, None])).scatter(1, y[:, None], 0.0)
+    R = rest.sum(1)
+    ez = (2 * (d / 32 + 40) + (8 if dtype == F32 else 0)) * ref.E32 * mag
+    rel = 2 * ez.max(1).values + (d + 4) * ref.E32 * mag.gather(1, y[:, None])[:, 0] + (300 + v / 8192) * ref.E32 + \
+        16 * ref.E32 * (z.abs().max(1).values + 1)
+    assert float(R.max()) < 0.3 and float(rel.max()) < 1e-3
+    tid = torch.stack([y, (y + 1) % v], 1)
+    sure = torch.tensor([[40.0, -80.0]], device=dev).expand(n, 2)             # q of the second: exp(-120) = 0 in 32 bits
+    for args in ((linear_cross_entropy, (y,)), (linear_distillation, (y[:, None], sure[:, :1])), (linear_distillation, (tid, sure))):
+        xr, wr = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+        loss = args[0](xr, wr, *args[1], reduction="none")
+        want = torch.log1p(R)
+        ref.assert_within("loss", loss.detach(), want, want * (rel + 8 * ref.E32) + 2.0 ** -126)
+        dx, _ = torch.autograd.grad(loss, (xr, wr), torch.ones(n, device=dev))
+        dz = (rest / (1 + R)[:, None]).scatter(1, y[:, None], (-R / (1 + R))[:, None])
+        u = ref.half_step(dtype)
+        # entries: their relative error, the rounding to the operands' type (fp16: the smallest numbers), the tail of three parts
+        e_dz = dz.abs() * (rel[:, None] + ez + u + 8 * ref.E32) + 4 * 2.0 ** -126 + (2.0 ** -25 / 4096 if dtype == F16 else 0.0)
+        exact = dz @ w.double()
+        bound = e_dz @ w.double().abs() + (2 * (v / 32 + 40) + 72) * ref.E32 * ((dz.abs() + e_dz) @ w.double().abs()) + u * exact.abs() + \
+            ref.floor_of(dtype)
+        ref.assert_within("dx", dx, exact, bound)
