@@ -16,7 +16,7 @@
 // (dx over the piece, dw of the piece).  A piece is at most DZ_BYTES: it is still in the last-level cache when it is read
 // (products at V = 131072: 1005 us; with 64 MB pieces, twice as many launches, 1267, with 256 MB 1273).
 //
-// Bound by the matrix units, and by what runs between products.  4096 x 32768 x 512 bf16: z 151 us (0.91 PF/s, about a quarter of
+// Bound by the matrix units, and by what runs between products.  4096 x 32768 x 512 bf16: z 152 us (0.90 PF/s, about a quarter of
 // it the exponentials), dz 174, the two products 275 (1.0 PF/s); matrix units busy half the cycles at 1.7-1.8 GHz.  32 rows or less are
 // bound by reading the codes: 16 x 65536 x 512 bf16 13.7 us (4.9 TB/s).
 //
@@ -457,7 +457,9 @@ __global__ void __launch_bounds__(TL::THREADS, TL::OCCUPANCY) head_walk_kernel(H
     Operand W, X;
     int64_t m0, n0;
     typename TL::Pipe pipe;
+    TileRows<TL, DZ> rows;
     head_tile<TL>(a, t, W, X, m0, n0);
+    if constexpr (!DZ) rows.request(a, n0);           // (before the tile's requests: the waits count what comes after)
     pipe.begin(W, X, a.nseg, ksteps, 0, steps, lds);
     // stores of dz by a wave behind the requests of its next tile (head_results: two per part, block of 64 classes and 16 rows)
     constexpr int STORES = DZ ? 2 * PARTS * (TL::MT / 4) * TL::NT : 0;
@@ -465,14 +467,13 @@ __global__ void __launch_bounds__(TL::THREADS, TL::OCCUPANCY) head_walk_kernel(H
     for (bool later = false;; later = true) {
         typename TL::Acc acc;
         clear<TL>(acc);
-        TileRows<TL, DZ> rows;
-        if constexpr (!DZ) rows.request(a, n0);
         pipe.template finish<STORES>(acc, later);
         rows.load(a, m0, n0);
         const int64_t m = m0, n = n0;
         t += stride;
         if (t < end) {
             head_tile<TL>(a, t, W, X, m0, n0);
+            if constexpr (!DZ) rows.request(a, n0);
             pipe.begin(W, X, a.nseg, ksteps, 0, steps, lds);
         }
         head_results<TL, DZ, PARTS>(a, acc, rows, m, n, part);
