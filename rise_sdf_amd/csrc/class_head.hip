@@ -42,6 +42,7 @@ constexpr int64_t DZ_BYTES = 128ll << 20;      // of one piece of dz
 // us of a step (64 deep) of a job of the products, and steps that a job costs beyond its own.  With 256 x 256 tiles alone 1000 x 10000 x
 // 200 bf16 took 90 us (here 76), with 128 x 128 ones 4096 x 32768 x 512 607 us (here 558); 0.45 to 0.65 chose alike but for long rows.
 constexpr double STEP_256 = 1.0, STEP_128 = 0.57, JOB_STEPS = 6.0;
+constexpr double PIECE = 15.0;
 constexpr int CUS = 256;                        // MI355X
 constexpr int64_t WPACK_BYTES = 128ll << 20;   // of the packed class codes of one piece
 
@@ -898,14 +899,16 @@ struct Plan {
 };
 
 // Tiles of z: 256 x 256, one per CU, or 128 x 128, two per CU.  Estimated us of a launch from what steps (64 deep) and results of a tile
-// took: the large ones come in whole rounds, the small ones fill the last one better (1000 x 20000 x 256 bf16: forward 18.4 against 22.9
+// took (dz writes its results too): the large ones come in whole rounds, the small ones fill the last one better (1000 x 20000 x 256 bf16: forward 18.4 against 22.9
 // us with large ones, backward 24.6 and 30.5; 1000 x 3000 x 100 fp32 11.2 and 21.4; but 4096 x 4096 x 256 fp32 57.5 and 40.8).
-bool by_quarters(int64_t n, int64_t classes, int64_t steps)
+struct Tiling { bool quarter; double us; };
+Tiling tiling(int64_t n, int64_t classes, int64_t steps, int dz_parts)
 {
     const int64_t large = (n + 255) / 256 * ((classes + 255) / 256), small = (n + 127) / 128 * ((classes + 127) / 128);
-    const double t256 = (double)((large + CUS - 1) / CUS) * (1.4 * steps + 5.0);
-    const double t128 = small <= CUS ? 0.7 * steps + 2.5 : (small <= 2 * CUS ? 1.0 : small / (2.0 * CUS) + 0.5) * (0.9 * steps + 2.5);
-    return t128 < t256;
+    const double t256 = (double)((large + CUS - 1) / CUS) * (1.4 * steps + 5.0 + 5.0 * dz_parts);
+    const double t128 = small <= CUS ? 0.7 * steps + 2.5 + 2.0 * dz_parts
+                                     : (small <= 2 * CUS ? 1.0 : small / (2.0 * CUS) + 0.5) * (0.9 * steps + 2.5 + 2.0 * dz_parts);
+    return Tiling{t128 < t256, t128 < t256 ? t128 : t256};
 }
 
 Plan make_plan(int64_t n, int64_t v, int d, int dtype)
@@ -926,11 +929,22 @@ Plan make_plan(int64_t n, int64_t v, int d, int dtype)
     p.vf = p.direct ? 256ll * ((1ll << 22) / ((n + 31) / 32)) : packed;
     if (p.vf < 256) p.vf = 256;
     p.vf = p.vf < up(v, 256) ? p.vf : up(v, 256);
-    const int64_t pieces = (v + most - 1) / most;
-    p.vc = up((v + pieces - 1) / pieces, 256);
     const int64_t steps = (int64_t)(p.parts == 3 ? 6 : 1) * (p.dp / 64);
-    p.quarter_fwd = by_quarters(n, p.vf < v ? p.vf : v, steps);
-    p.quarter_bwd = by_quarters(n, p.vc < v ? p.vc : v, steps);
+    p.quarter_fwd = tiling(n, p.vf < v ? p.vf : v, steps, 0).quarter;
+    // backward: as few pieces as fit, or more where their tiles come in whole rounds (PIECE us: the launches around a piece).  With gradients,
+    // against as few as fit: 3000 x 131000 x 256 bf16 1050 and 1109 us, 1644 x 72779 x 176 fp32 1452 and 1486, 7000 x 70000 x 64 fp16 879 and 906
+    const int64_t blocks = (v + 255) / 256, fewest = (v + most - 1) / most;
+    double least = 0.0;
+    for (int64_t pieces = fewest; pieces <= 2 * fewest && pieces <= fewest + 32; ++pieces) {
+        const int64_t each = (blocks + pieces - 1) / pieces;
+        const Tiling t = tiling(n, each * 256 < v ? each * 256 : v, steps, p.parts);
+        const double us = (double)((blocks + each - 1) / each) * (t.us + PIECE);
+        if (least == 0.0 || us < least) {
+            least = us;
+            p.vc = each * 256;
+            p.quarter_bwd = t.quarter;
+        }
+    }
     p.sbm = p.quarter_fwd && !p.small ? 128 : 256;
     // The products of a piece are cut over k into jobs of about `job` steps (64 deep), by tiles of 256 x 256 (one per CU) or
     // 128 x 128 (two); what has the least estimated time is taken.  In us: a job's steps and its own cost (its first
