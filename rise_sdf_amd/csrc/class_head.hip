@@ -569,100 +569,102 @@ __global__ void __launch_bounds__(256) rows_kernel(RowArgs a)
     __shared__ float part[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t r0 = (int64_t)blockIdx.x * LR;
-    {
-        const int r = tid % LR;
-        float2 s = {-__builtin_inff(), 0.0f};
-        if (r0 + r < a.n)
-            for (int64_t t = tid / LR; t < a.tiles; t += 256 / LR) s = join_stats(s, a.stats[t * a.n + r0 + r]);
-        st[tid] = s;
+    const int rr = LR == 1 ? 0 : wave;
+    const int64_t r = r0 + rr;
+    const bool there = r < a.n;                     // (LR 1: always)
+    const float inv_t = 1.0f / a.temperature, c = LOG2E * inv_t;
+    // the statistics are on their way while the first class's logit is computed
+    const int sr = tid % LR;
+    int64_t t = tid / LR;
+    const int64_t stat_rows = r0 + sr < a.n ? a.tiles : 0;
+    float2 s = t < stat_rows ? a.stats[t * a.n + r0 + sr] : float2{-__builtin_inff(), 0.0f};
+    const int64_t first = there ? a.ids[r * a.k] : -1;
+    const bool pivot = first >= 0 && first < a.v && (a.logits != nullptr || first != a.ignore);
+    const float zp = pivot ? dot<DT, BYTES>(a.x, a.w, r * a.d, first * a.d, a.d) : 0.0f;
+    for (t += 256 / LR; t < stat_rows; t += 256 / LR) s = join_stats(s, a.stats[t * a.n + r0 + sr]);
+    st[tid] = s;
+    __syncthreads();
+    for (int o = 128; o >= LR; o >>= 1) {
+        if (tid < o) st[tid] = join_stats(st[tid], st[tid + o]);
         __syncthreads();
-        for (int o = 128; o >= LR; o >>= 1) {
-            if (tid < o) st[tid] = join_stats(st[tid], st[tid + o]);
-            __syncthreads();
-        }
     }
-    const float inv_t = 1.0f / a.temperature;
-    for (int rr = LR == 1 ? 0 : wave; rr < LR; rr += 4) {
-        const int64_t r = r0 + rr;
-        if (r >= a.n) return;                       // (LR 1: r0 < n)
-        const float c = LOG2E * inv_t;
-        const int64_t first = a.ids[r * a.k];
-        // lse = ref + over in powers of two, kept apart: with a first class, over = log(1 + what is smaller, it or the others)
-        const bool pivot = first >= 0 && first < a.v && (a.logits != nullptr || first != a.ignore);
-        const float zp = pivot ? dot<DT, BYTES>(a.x, a.w, r * a.d, first * a.d, a.d) : 0.0f;
-        const float rest = st[rr].x + __builtin_amdgcn_logf(st[rr].y);    // v_log_f32: base 2
-        const float u = zp * c - rest, near = __builtin_amdgcn_exp2f(-fabsf(u));
-        const float ref = pivot ? fmaxf(zp * c, rest) : st[rr].x;
-        const float over = pivot ? log1pf(near) * LOG2E : __builtin_amdgcn_logf(st[rr].y);
-        const float miss = pivot ? 1.0f / (1.0f + __builtin_amdgcn_exp2f(u)) : 1.0f;
-        float lse = ref + over;
-        if (!(fabsf(lse) < __builtin_inff())) lse = __builtin_nanf("");   // (+inf means something else)
-        float loss = 0.0f;
-        bool alive = false, bad = false;
-        if (a.logits == nullptr) {
-            bad = first != a.ignore && !pivot;
-            alive = pivot;
-            if (alive) loss = ((ref - zp * c) + over) * LN2 + (lse - lse);
-        } else {
-            const int64_t *ids = a.ids + r * a.k;
-            const float *lg = a.logits + r * a.k;
-            float *q = a.q + r * a.k, *zt = a.zt + r * a.k;
-            float tm = -__builtin_inff();
-            bool nan = false;
-            for (int k = lane; k < a.k; k += 64) {
-                if (ids[k] < 0) continue;           // (whatever its logit holds)
-                bad |= ids[k] >= a.v;
-                nan |= lg[k] != lg[k];
-                tm = fmaxf(tm, lg[k]);
+    if (!there) return;
+    // lse = ref + over in powers of two, kept apart: with a first class, over = log(1 + what is smaller, it or the others)
+    const float rest = st[rr].x + __builtin_amdgcn_logf(st[rr].y);    // v_log_f32: base 2
+    const float u = zp * c - rest, near = __builtin_amdgcn_exp2f(-fabsf(u));
+    const float ref = pivot ? fmaxf(zp * c, rest) : st[rr].x;
+    const float over = pivot ? log1pf(near) * LOG2E : __builtin_amdgcn_logf(st[rr].y);
+    const float miss = pivot ? 1.0f / (1.0f + __builtin_amdgcn_exp2f(u)) : 1.0f;
+    float lse = ref + over;
+    if (!(fabsf(lse) < __builtin_inff())) lse = __builtin_nanf("");   // (+inf means something else)
+    float loss = 0.0f;
+    bool alive = false, bad = false;
+    if (a.logits == nullptr) {
+        bad = first != a.ignore && !pivot;
+        alive = pivot;
+        if (alive) loss = ((ref - zp * c) + over) * LN2 + (lse - lse);
+    } else {
+        const int64_t *ids = a.ids + r * a.k;
+        const float *lg = a.logits + r * a.k;
+        float *q = a.q + r * a.k, *zt = a.zt + r * a.k;
+        float tm = -__builtin_inff();
+        bool nan = false;
+        for (int k = lane; k < a.k; k += 64) {
+            if (ids[k] < 0) continue;           // (whatever its logit holds)
+            bad |= ids[k] >= a.v;
+            nan |= lg[k] != lg[k];
+            tm = fmaxf(tm, lg[k]);
+        }
+        tm = wave_max(tm);
+        bad = __any(bad);
+        alive = (tm > -__builtin_inff() || __any(nan)) && !bad;
+        float sum = 0.0f;
+        if (alive)
+            for (int k = lane; k < a.k; k += 64)
+                if (ids[k] >= 0) sum += expf((lg[k] - tm) * inv_t);   // (the difference first: logits at the type's ends)
+        sum = wave_sum(sum);
+        const float ls = logf(sum);
+        int listed = 0;                                               // of 64 entries; for an absent one a class that is there
+        for (int k0 = LR == 1 ? wave * G : 0; k0 < a.k; k0 += LR == 1 ? 4 * G : G) {
+            if ((k0 & 63) < (LR == 1 ? 4 * G : G)) {
+                const int k = (k0 & ~63) + lane;
+                const int64_t id = k < a.k ? ids[k] : -1;
+                listed = alive && id >= 0 ? (int)id : 0;
             }
-            tm = wave_max(tm);
-            bad = __any(bad);
-            alive = (tm > -__builtin_inff() || __any(nan)) && !bad;
-            float sum = 0.0f;
-            if (alive)
-                for (int k = lane; k < a.k; k += 64)
-                    if (ids[k] >= 0) sum += expf((lg[k] - tm) * inv_t);   // (the difference first: logits at the type's ends)
-            sum = wave_sum(sum);
-            const float ls = logf(sum);
-            for (int k0 = LR == 1 ? wave * G : 0; k0 < a.k; k0 += LR == 1 ? 4 * G : G) {
-                int64_t wo[G];
+            int64_t wo[G];
 #pragma unroll
-                for (int j = 0; j < G; ++j) {
-                    const int64_t id = k0 + j < a.k ? ids[k0 + j] : -1;
-                    wo[j] = (alive && id >= 0 ? id : 0) * a.d;            // (a class that is there; its product is not used)
+            for (int j = 0; j < G; ++j) wo[j] = (int64_t)__builtin_amdgcn_readlane(listed, (k0 & 63) + j) * a.d;
+            float z = alive ? dots<DT, BYTES>(a.x, a.w, r * a.d, wo, a.d) : 0.0f;
+            const int k = k0 + ((lane >> 3) & 7);
+            if (k < a.k && (lane & 7) == 0) {
+                float qk = 0.0f;
+                if (alive && ids[k] >= 0) {
+                    if (ids[k] == first) z = zp;
+                    const float lq = (lg[k] - tm) * inv_t - ls;
+                    qk = expf(lq);
+                    if (!(qk == 0.0f)) loss += qk * (lq + ((ref - z * c) + over) * LN2) + (lse - lse);
+                } else {
+                    z = 0.0f;
                 }
-                float z = alive ? dots<DT, BYTES>(a.x, a.w, r * a.d, wo, a.d) : 0.0f;
-                const int k = k0 + ((lane >> 3) & 7);
-                if (k < a.k && (lane & 7) == 0) {
-                    float qk = 0.0f;
-                    if (alive && ids[k] >= 0) {
-                        if (ids[k] == first) z = zp;
-                        const float lq = (lg[k] - tm) * inv_t - ls;
-                        qk = expf(lq);
-                        if (!(qk == 0.0f)) loss += qk * (lq + ((ref - z * c) + over) * LN2) + (lse - lse);
-                    } else {
-                        z = 0.0f;
-                    }
-                    q[k] = qk;
-                    zt[k] = z;
-                }
+                q[k] = qk;
+                zt[k] = z;
             }
-            loss = wave_sum(loss);
-            if (LR == 1) {
-                if (lane == 0) part[wave] = loss;
-                __syncthreads();
-                loss = (part[0] + part[1]) + (part[2] + part[3]);
-                if (wave != 0) return;
-            }
-            loss *= a.temperature * a.temperature;
         }
-        if (lane == 0) {
-            if (bad) loss = __builtin_nanf("");
-            if (bad && a.status != nullptr) atomicAdd(a.status, 1);
-            a.loss[r] = loss;
-            a.lse[r] = alive ? lse : __builtin_inff();
-            a.lse[a.n + r] = miss;
+        loss = wave_sum(loss);
+        if (LR == 1) {
+            if (lane == 0) part[wave] = loss;
+            __syncthreads();
+            loss = (part[0] + part[1]) + (part[2] + part[3]);
+            if (wave != 0) return;
         }
+        loss *= a.temperature * a.temperature;
+    }
+    if (lane == 0) {
+        if (bad) loss = __builtin_nanf("");
+        if (bad && a.status != nullptr) atomicAdd(a.status, 1);
+        a.loss[r] = loss;
+        a.lse[r] = alive ? lse : __builtin_inff();
+        a.lse[a.n + r] = miss;
     }
 }
 
@@ -898,9 +900,10 @@ struct Plan {
     bool x_first;                    // the jobs of dx are the longer ones
 };
 
-// Tiles of z: 256 x 256, one per CU, or 128 x 128, two per CU.  Estimated us of a launch from what steps (64 deep) and results of a tile
-// took (dz writes its results too): the large ones come in whole rounds, the small ones fill the last one better (1000 x 20000 x 256 bf16: forward 18.4 against 22.9
-// us with large ones, backward 24.6 and 30.5; 1000 x 3000 x 100 fp32 11.2 and 21.4; but 4096 x 4096 x 256 fp32 57.5 and 40.8).
+// Tiles of z: 256 x 256, one per CU, or 128 x 128, two per CU.  Estimated us of a launch from what steps (64 deep) and results of a
+// tile took (dz writes its results too): the large ones come in whole rounds, the small ones fill the last one better (1000 x 20000 x
+// 256 bf16: forward 18.4 against 22.9 us with large ones, backward 24.6 and 30.5; 1000 x 3000 x 100 fp32 11.2 and 21.4; but 4096 x
+// 4096 x 256 fp32 57.5 and 40.8).
 struct Tiling { bool quarter; double us; };
 Tiling tiling(int64_t n, int64_t classes, int64_t steps, int dz_parts)
 {
