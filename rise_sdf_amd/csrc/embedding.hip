@@ -61,7 +61,8 @@ template <bool NT, class V, class T> __device__ __forceinline__ void store_at(T 
 }
 
 // ---- lookup -------------------------------------------------------------------------------------------------------------------
-// NT: the output passes the caches by (262144 x 256 bf16: 28 instead of 42 us, and the table stays in them)
+// NT: the output passes the caches by, the table stays in them (262144 x 256 bf16: 28 instead of 42 us where few ids are frequent, 39 and 40
+// where all are alike; 10000 x 100 fp16 3.5 and 3.4; with a reader right behind it 4 to 128 MB differ by less than 5 % either way)
 template <int DT, int VW, bool NT>
 __global__ void __launch_bounds__(256) lookup_kernel(const int64_t *__restrict__ ids, int64_t n, const void *__restrict__ table, int64_t v,
                                                      int d, int per_row, float scale, int64_t padding, int rows_per_block,
