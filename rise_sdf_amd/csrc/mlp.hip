@@ -34,9 +34,9 @@ constexpr int S_THREADS = S_WAVES * 64;
 #ifndef RSDF_LIN_KSU_BI
 #define RSDF_LIN_KSU_BI 4
 #endif
-// Weight gradient of a layer with K <= 64 input columns: capped at 128 registers (24 bytes of scratch) so that two
-// workgroups share a CU: 1.14 -> 0.83 ms (35x64), 1.19 -> 0.91 (64x64).  The wide instantiations spill badly under the same
-// cap (10-15 ms) and keep one workgroup per CU.
+// Weight gradient of a layer with K <= 64 input columns: two workgroups share a CU (128 registers; it needs 93 and spills none).
+// 4 M rows, kernels alone, a row's address shared by its lanes against one per lane (9 registers spilled at K <= 64):
+//   35x64 0.76 -> 0.35 ms, 64x64 0.79 -> 0.38, 84x128 1.54 -> 0.91, 128x128 2.03 -> 1.13, 128x6 0.59 -> 0.37
 #ifndef RSDF_BWDW_OCC
 #define RSDF_BWDW_OCC 4
 #endif
@@ -247,7 +247,7 @@ linear_bwd_weight_kernel(const float *__restrict__ dz, int lddz, const float *__
                          int ldx, int64_t n, int K, int N, float *__restrict__ dw,
                          float *__restrict__ db)
 {
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 31, hf = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63, c = lane & 31, hf = lane >> 5;
     const int NT = (N + 31) >> 5;
     const int slabs = S_WAVES / NT;              // row slabs per workgroup (waves beyond NT * slabs idle)
     const int nt = wave % NT, slab = wave / NT;
@@ -260,24 +260,44 @@ linear_bwd_weight_kernel(const float *__restrict__ dz, int lddz, const float *__
     float bsum = 0.0f;
     const int ncol = nt * 32 + c;
     const bool nok = ncol < N;
-    const int64_t n_steps = (n + 15) >> 4;       // 16 rows per MFMA k-step
-    const int64_t stride = (int64_t)gridDim.x * slabs;
-    for (int64_t step = (int64_t)blockIdx.x * slabs + slab; step < n_steps; step += stride) {
-        const int64_t r0 = step * 16 + 8 * hf;
-        float av[8];
+    // A load's address is a row (the same for all lanes) plus a lane's own offset, which every row shares.  Lanes beyond the last column
+    // read that column again: what they add up belongs to no output.
+    const unsigned zo = (unsigned)(8 * hf * lddz + (nok ? ncol : N - 1));
+    unsigned xo[KT];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) av[j] = (nok && r0 + j < n) ? dz[(r0 + j) * lddz + ncol] : 0.0f;
+    for (int t = 0; t < KT; ++t) xo[t] = (unsigned)(8 * hf * ldx + (t * 32 + c < K ? t * 32 + c : K - 1));
+    auto add = [&](const float (&av)[8], const float (&bv)[KT][8]) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) bsum += av[j];
         const Frag3 af = split_frag(av[0], av[1], av[2], av[3], av[4], av[5], av[6], av[7]);
 #pragma unroll
-        for (int t = 0; t < KT; ++t) {
-            const int kcol = t * 32 + c;
-            float bv[8];
+        for (int t = 0; t < KT; ++t)
+            acc[t] = mma6r(af, split_frag(bv[t][0], bv[t][1], bv[t][2], bv[t][3], bv[t][4], bv[t][5], bv[t][6], bv[t][7]), acc[t]);
+    };
+    const int64_t n_steps = n >> 4, stride = (int64_t)gridDim.x * slabs;       // whole steps of 16 rows: one MFMA k-step
+    int64_t step = (int64_t)blockIdx.x * slabs + slab;
+    for (; step < n_steps; step += stride) {
+        const float *zr = dz + step * 16 * lddz, *xr = x + step * 16 * ldx;
+        float av[8], bv[KT][8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) bv[j] = (kcol < K && r0 + j < n) ? x[(r0 + j) * ldx + kcol] : 0.0f;
-            acc[t] = mma6r(af, split_frag(bv[0], bv[1], bv[2], bv[3], bv[4], bv[5], bv[6], bv[7]), acc[t]);
-        }
+        for (int j = 0; j < 8; ++j) av[j] = (zr + j * lddz)[zo];
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) bv[t][j] = (xr + j * ldx)[xo[t]];
+        add(av, bv);
+    }
+    if (step == n_steps && (n & 15) != 0) {      // the last rows
+        const float *zr = dz + step * 16 * lddz, *xr = x + step * 16 * ldx;
+        const int left = (int)(n & 15) - 8 * hf;
+        float av[8], bv[KT][8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) av[j] = j < left ? (zr + j * lddz)[zo] : 0.0f;
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) bv[t][j] = j < left ? (xr + j * ldx)[xo[t]] : 0.0f;
+        add(av, bv);
     }
     // The row slabs of the workgroup meet in LDS, slab by slab, and slab 0 flushes: one add per workgroup and address.  A
     // narrow output layer (N <= 4: eight slabs, 512 workgroups) used to send 4096 float atomics to each of its few dw / db
