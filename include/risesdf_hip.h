@@ -729,7 +729,7 @@ int rsdf_embedding_bwd(const int64_t *ids, int64_t n, const void *grad, int64_t 
  * listed id outside [0, v) makes its row's loss NaN, adds nothing to the gradients and is counted into *bad_ids (nullable,
  * accumulates).
  * fwd: reduction 0: loss [n]; 1: loss [1] = mean over the rows that take part (0 without any), count [1] = their number (at
- *   least 1); 2: loss [1] = sum.  lse [2][n] (log-sum-exp in powers of two; 1 - the probability
+ *   least 1); 2: loss [1] = sum (count nullable, written if there).  lse [2][n] (log-sum-exp in powers of two; 1 - the probability
  *   of the first listed class), q [n][k] and listed_z [n][k] (teacher only) are what bwd reads.
  * bwd: grad = d(loss): [n] (grad_per_row) or [1]; count as written by fwd for reduction 1, else NULL.  dx [n][d] / dw [v][d]
  *   (nullable: not computed).

@@ -688,7 +688,7 @@ __global__ void __launch_bounds__(1024) sum_kernel(const float *__restrict__ los
         for (int i = 0; i < 16; ++i) { l += sl[i]; c += sc[i]; }
         c = c > 1.0 ? c : 1.0;
         out[0] = (float)(mean ? l / c : l);
-        count[0] = (float)c;
+        if (count != nullptr) count[0] = (float)c;
     }
 }
 
@@ -1172,10 +1172,12 @@ int rsdf_class_head_fwd(const void *x, const void *w, int64_t n, int64_t v, int 
     RSDF_CHECK_ARG(teacher_logits != nullptr ? (q != nullptr && listed_z != nullptr) : k == 1,
                    "class_head_fwd: a teacher needs q and listed_z, labels need k = 1");
     RSDF_CHECK_ARG(reduction >= 0 && reduction <= 2, "class_head_fwd: reduction must be 0 (none), 1 (mean) or 2 (sum)");
+    RSDF_CHECK_ARG(x != nullptr && w != nullptr && ids != nullptr && loss != nullptr && lse != nullptr && (count != nullptr || reduction != 1),
+                   "class_head_fwd: x, w, ids, loss, lse, and for a mean count, must not be NULL");
     const Plan p = make_plan(n, v, d, dtype);
     Space s{(unsigned char *)workspace};
     const FwdSpace f = fwd_space(p, s);
-    RSDF_CHECK_ARG(s.at <= workspace_bytes, "class_head_fwd: workspace too small");
+    RSDF_CHECK_ARG(workspace != nullptr && s.at <= workspace_bytes, "class_head_fwd: workspace too small");
     hipStream_t st = (hipStream_t)stream;
     const int64_t xplane = p.n_pad * p.dp, wplane = p.vf * p.dp;
     for (int64_t v0 = 0; v0 < v; v0 += p.vf) {
@@ -1215,12 +1217,14 @@ int rsdf_class_head_bwd(const void *x, const void *w, int64_t n, int64_t v, int 
     RSDF_CHECK_ARG(bad == nullptr, bad);
     RSDF_CHECK_ARG((q == nullptr) == (listed_z == nullptr) && (q != nullptr || k == 1),
                    "class_head_bwd: a teacher needs q and listed_z, labels need k = 1");
+    RSDF_CHECK_ARG(x != nullptr && w != nullptr && ids != nullptr && lse != nullptr && grad != nullptr,
+                   "class_head_bwd: x, w, ids, lse and grad must not be NULL");
     RSDF_CHECK_ARG((((uintptr_t)dx | (uintptr_t)dw) & 15) == 0, "class_head_bwd: dx and dw must be 16-byte aligned");
     if (dx == nullptr && dw == nullptr) return 0;
     const Plan p = make_plan(n, v, d, dtype);
     Space s{(unsigned char *)workspace};
     const BwdSpace b = bwd_space(p, s, dx != nullptr, dw != nullptr);
-    RSDF_CHECK_ARG(s.at <= workspace_bytes, "class_head_bwd: workspace too small");
+    RSDF_CHECK_ARG(workspace != nullptr && s.at <= workspace_bytes, "class_head_bwd: workspace too small");
     hipStream_t st = (hipStream_t)stream;
     const int nseg = p.parts == 3 ? 6 : 1;
     const int64_t xplane = p.n_pad * p.dp, wplane = p.vc * p.dp, zplane = p.n_pad * p.vc;

@@ -575,6 +575,7 @@ int rsdf_embedding_fwd(const int64_t *ids, int64_t n, const void *table, int64_t
     const char *bad = bad_shape(n, v, d, dtype);
     RSDF_CHECK_ARG(bad == nullptr, bad);
     if (n == 0) return 0;
+    RSDF_CHECK_ARG(ids != nullptr && table != nullptr && out != nullptr, "embedding_fwd: ids, table and out must not be NULL");
     const int bytes = vector_bytes(d, dtype), size = dtype == T_F32 ? 4 : 2;
     const int per_row = (d * size + bytes - 1) / bytes;
     int rows = 1024 / per_row;                          // about four vectors a thread
@@ -601,6 +602,8 @@ int rsdf_embedding_bwd(const int64_t *ids, int64_t n, const void *grad, int64_t 
 {
     const char *bad = bad_shape(n, v, d, dtype);
     RSDF_CHECK_ARG(bad == nullptr, bad);
+    RSDF_CHECK_ARG(d_table != nullptr && (n == 0 || (ids != nullptr && grad != nullptr)),
+                   "embedding_bwd: d_table, and with positions ids and grad, must not be NULL");
     hipStream_t st = (hipStream_t)stream;
     const int bytes = vector_bytes(d, dtype), size = dtype == T_F32 ? 4 : 2;
     const int per_row = (d * size + bytes - 1) / bytes;
@@ -614,7 +617,7 @@ int rsdf_embedding_bwd(const int64_t *ids, int64_t n, const void *grad, int64_t 
         RSDF_RETURN_LAUNCH();
     }
     const Space s = space(workspace, n, v, d);
-    RSDF_CHECK_ARG(s.bytes <= workspace_bytes, "embedding_bwd: workspace too small");
+    RSDF_CHECK_ARG(workspace != nullptr && s.bytes <= workspace_bytes, "embedding_bwd: workspace too small");
     const Sorting so = sorting(n, v);
     int from = 1;
     if (n > 0)
