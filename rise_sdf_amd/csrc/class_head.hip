@@ -501,7 +501,7 @@ struct RowArgs {
 // together, so that they cost 10 exchanges instead of 48.
 constexpr int G = 8;
 template <int E> struct Words { using type = u32x4; };
-template <> struct Words<8> { using type = uint2; };
+template <> struct Words<8> { using type = __attribute__((ext_vector_type(2))) unsigned; };
 template <> struct Words<4> { using type = unsigned; };
 template <int DT, int BYTES>
 __device__ __forceinline__ float dots(const void *x, const void *w, int64_t xo, const int64_t (&wo)[G], int d)
