@@ -19,7 +19,8 @@ def check_status(device=None) -> dict:
     """Reads the kernels' sticky status words (one small device-to-host copy; blocks on the device).  If a kernel of the
     two-part fp16 number format left its range since the last check, that kernel family is switched to the range-free
     kernels for the rest of the process with a RuntimeWarning (``rerouted_now`` in the result; RSDF_RANGE_ERROR=raise:
-    RiseSdfHipError instead); returns the counters (``x2_bwd_rerouted``: backward launches the range guard ran on the range-free kernels).  The
+    RiseSdfHipError instead); returns the counters (``x2_bwd_rerouted``: backward launches the range guard ran on the range-free kernels).  Ids, labels or listed classes
+    outside their table since the last check (ops.embedding, the losses of a linear head) raise RiseSdfHipError.  The
     samplers call this themselves behind the host reads they make anyway; call it after a loop that makes none."""
     from . import _lib
     return _lib.poll_status(device)

@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import threading
 
 import torch
 
@@ -450,6 +451,7 @@ STATUS_WORDS = 8
 ST_X2_FWD_NONFINITE, ST_X2_BWD_REROUTED, ST_X2_BWD_GUARDED, ST_PAIR_PACK_NONFINITE, ST_PAIR_FWD_NONFINITE = 0, 1, 2, 3, 4
 ST_BAD_IDS = 5
 _STATUS = {}
+_STATUS_LOCK = threading.Lock()        # the words' creation, and what the polls have seen
 _STATUS_SEEN = {}        # device index -> the raw words at the last poll (the device-side words are MONOTONIC: never cleared)
 _STATUS_TOTALS = {"x2_bwd_rerouted": 0, "x2_bwd_guarded": 0, "x2_fwd_nonfinite_total": 0, "range_reroutes": 0,
                   "bad_ids": 0}
@@ -485,9 +487,15 @@ def status(device) -> "torch.Tensor":
     idx = dev.index if dev.index is not None else torch.cuda.current_device()
     t = _STATUS.get(idx)
     if t is None:
-        t = torch.zeros(STATUS_WORDS, dtype=torch.int32, device=torch.device("cuda", idx))
-        _STATUS[idx] = t
-        _STATUS_SEEN[idx] = [0] * STATUS_WORDS
+        with _STATUS_LOCK:
+            t = _STATUS.get(idx)
+            if t is None:
+                with torch.cuda.device(idx):
+                    t = torch.zeros(STATUS_WORDS, dtype=torch.int32, device=torch.device("cuda", idx))
+                    if not torch.cuda.is_current_stream_capturing():
+                        torch.cuda.current_stream().synchronize()     # (any stream may count into them next)
+                _STATUS_SEEN[idx] = [0] * STATUS_WORDS
+                _STATUS[idx] = t
     return t
 
 
@@ -499,18 +507,22 @@ def bad_ids_ptr(idx):
     captured on a device that has no status words yet: they would live in the graph's private pool."""
     p = _BAD_IDS_PTR.get(idx)
     if p is None:
-        if idx not in _STATUS and torch.cuda.is_current_stream_capturing():
+        with torch.cuda.device(idx):
+            capturing = torch.cuda.is_current_stream_capturing()
+        if idx not in _STATUS and capturing:
             return 0
         p = _BAD_IDS_PTR[idx] = status(torch.device("cuda", idx)).data_ptr() + 4 * ST_BAD_IDS
     return p
 
 
 def _status_delta(idx, vals):
-    """Counts since the last poll of device ``idx`` (wrap-around safe), and remember ``vals`` as seen."""
-    seen = _STATUS_SEEN.setdefault(idx, [0] * STATUS_WORDS)
-    d = [((int(v) - int(s)) + (1 << 31)) % (1 << 32) - (1 << 31) for v, s in zip(vals, seen)]
-    _STATUS_SEEN[idx] = [int(v) for v in vals]
-    return d
+    """Counts since the last poll of device ``idx`` (wrap-around safe), and remember ``vals`` as seen.  The words only grow: ones that were
+    read before another thread's poll, and get here after it, hold nothing new."""
+    with _STATUS_LOCK:
+        seen = _STATUS_SEEN.setdefault(idx, [0] * STATUS_WORDS)
+        d = [((int(v) - int(s)) + (1 << 31)) % (1 << 32) - (1 << 31) for v, s in zip(vals, seen)]
+        _STATUS_SEEN[idx] = [int(v) if n > 0 else s for v, s, n in zip(vals, seen, d)]
+        return [max(n, 0) for n in d]
 
 
 def poll_status(device=None, raise_on_error=True) -> dict:
@@ -553,6 +565,12 @@ def _range_message(bad, sites):
             "|input|, |weight| or a hidden activation >= 1023 -- where the reference's fp32 MLPs stay finite.")
 
 
+def _ids_message(ids):
+    return (f"{ids} rows named an id outside the table (ops.embedding) or a label / listed class outside the "
+            "head (loss.linear_cross_entropy, loss.linear_distillation) since the last check: their "
+            "outputs are NaN and they took no part in the gradients")
+
+
 def _status_result(bad, raise_on_error, sites=(0, 0), ids=0):
     rerouted = False
     _STATUS_TOTALS["bad_ids"] += ids
@@ -561,7 +579,7 @@ def _status_result(bad, raise_on_error, sites=(0, 0), ids=0):
         if raise_on_error and range_policy() == "raise":
             raise RiseSdfHipError(
                 _range_message(bad, sites) + "  Set RSDF_X2=0 (SDF network) / RSDF_PAIR=0 (radiance networks) to run on the "
-                "range-free kernels (three bf16 parts, fp32's exponent range).")
+                "range-free kernels (three bf16 parts, fp32's exponent range)." + ("  Also: " + _ids_message(ids) if ids else ""))
         if raise_on_error:
             import warnings
             kinds = [k for k, n in (("x2", bad - sites[0] - sites[1]), ("pair", sites[0] + sites[1])) if n > 0 and not _RANGE_FREE[k]]
@@ -577,9 +595,7 @@ def _status_result(bad, raise_on_error, sites=(0, 0), ids=0):
                     "rise_sdf_amd.guarded, TrainStep skips that optimizer step).  RSDF_RANGE_ERROR=raise raises instead.",
                     RuntimeWarning, stacklevel=3)
     if ids and raise_on_error:
-        raise RiseSdfHipError(f"{ids} rows named an id outside the table (ops.embedding) or a label / listed class outside the "
-                              "head (loss.linear_cross_entropy, loss.linear_distillation) since the last check: their "
-                              "outputs are NaN and they took no part in the gradients")
+        raise RiseSdfHipError(_ids_message(ids))
     return dict(_STATUS_TOTALS, x2_fwd_nonfinite=bad, rerouted_now=rerouted)
 
 
