@@ -7,8 +7,11 @@
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
+
+#include <unordered_set>
 
 namespace {
 
@@ -51,20 +54,42 @@ Tensor bytes_on(int64_t n, const Tensor &like)
 
 template <class T> T *address(const Tensor &t) { return t.defined() ? (T *)t.data_ptr() : nullptr; }
 
-// A leaf remembers the stream on which a graph that is still alive first used it, and its gradient is accumulated there.  Inside a
-// capture that would tie an eager stream to the captured one, which ends the process, so the call is refused while it can be.
-void check_leaf(const Tensor &t, const char *what)
+// whether a stream of this device is being captured
+bool captured(const c10::Stream &s)
 {
-    if (!at::GradMode::is_enabled() || !t.requires_grad() || !t.is_leaf()) return;
+    if (s.id() == c10::hip::getDefaultHIPStream(s.device_index()).id()) return false;
+    const c10::DeviceGuard guard(c10::Device(c10::DeviceType::CUDA, s.device_index()));
+    const auto now = c10::hip::getCurrentHIPStream(s.device_index());
+    c10::hip::setCurrentHIPStream(c10::hip::HIPStream(
+        c10::hip::HIPStream::UNCHECKED, c10::Stream(c10::Stream::UNSAFE, c10::Device(c10::DeviceType::HIP, s.device_index()), s.id())));
+    const bool yes = c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None;
+    c10::hip::setCurrentHIPStream(now);
+    return yes;
+}
+
+// A leaf remembers the stream on which a graph that is still alive first used it, and its gradient is accumulated there.  Inside a
+// capture that would tie an eager stream to the captured one, which ends the process, so the call is refused while it can be.  All
+// leaves behind the operand count: it may be a view, a cast or a layer's output.
+void check_leaves(const Tensor &t, const char *what)
+{
+    if (!at::GradMode::is_enabled() || !t.requires_grad()) return;
     const c10::DeviceGuard guard(t.device());
     if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
-    const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
-    if (node == nullptr) return;
-    const auto there = node->stream();
-    // (by id: one of the two calls the device HIP, the other CUDA)
-    if (there.has_value() && there->id() != c10::hip::getCurrentHIPStream(t.get_device()).id())
-        throw Error(std::string(what) + ": a leaf of this captured pass is part of a graph that was recorded on another stream and is "
-                    "still alive; drop that graph (its outputs and losses) before the capture");
+    const auto node = t.is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(t) : t.grad_fn();
+    std::vector<torch::autograd::Node *> todo{node.get()};
+    std::unordered_set<torch::autograd::Node *> seen;
+    while (!todo.empty()) {
+        auto *n = todo.back();
+        todo.pop_back();
+        if (n == nullptr || !seen.insert(n).second) continue;
+        for (const auto &e : n->next_edges()) todo.push_back(e.function.get());
+        if (dynamic_cast<torch::autograd::AccumulateGrad *>(n) == nullptr) continue;
+        const auto there = n->stream();
+        // (by id: one of the two calls the device HIP, the other CUDA)
+        if (there.has_value() && there->id() != c10::hip::getCurrentHIPStream(there->device_index()).id() && !captured(*there))
+            throw Error(std::string(what) + ": a leaf of this captured pass is part of a graph that was recorded on another stream and is "
+                        "still alive; drop that graph (its outputs and losses) before the capture");
+    }
 }
 
 // gradients of a node that cannot be differentiated again: under create_graph a second derivative raises instead of being zero
@@ -213,14 +238,14 @@ PYBIND11_MODULE(_codebook, m)
     m.def("bind", &bind);
     m.def("embedding", [](const Tensor &ids, const Tensor &table, double scale, int64_t padding, int64_t bad_ids) {
         py::gil_scoped_release free;
-        check_leaf(table, "embedding");
+        check_leaves(table, "embedding");
         return Embedding::apply(ids, table, scale, padding, bad_ids);
     });
     m.def("class_head", [](const Tensor &x, const Tensor &w, const Tensor &ids, const c10::optional<Tensor> &logits, int64_t k, int64_t ignore,
                            double temperature, int64_t reduction, int64_t bad_ids) {
         py::gil_scoped_release free;
-        check_leaf(x, "the losses of a linear head");
-        check_leaf(w, "the losses of a linear head");
+        check_leaves(x, "the losses of a linear head");
+        check_leaves(w, "the losses of a linear head");
         return ClassHead::apply(x, w, ids, logits, k, ignore, temperature, reduction, bad_ids);
     });
 }
