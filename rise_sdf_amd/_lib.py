@@ -289,18 +289,23 @@ def set_timer(timer):
     """Install (or with None remove) a KernelTimer."""
     global _timer
     _timer = timer
+    _watch_nodes()
 
 
 _DEBUG_SYNC = os.environ.get("RSDF_DEBUG_SYNC", "")      # a file path: every entry point is logged there, then waited for
 
 
+def _debug_sync(what):
+    # debug aid for GPU memory faults (they abort the process from another thread, asynchronously): name the entry point
+    # BEFORE waiting for it, so that the last line of the file is the launch that faulted
+    with open(_DEBUG_SYNC, "a") as f:
+        f.write(what + "\n")
+    torch.cuda.synchronize()
+
+
 def check(rc: int, what: str):
     if _DEBUG_SYNC:
-        # debug aid for GPU memory faults (they abort the process from another thread, asynchronously): name the entry point
-        # BEFORE waiting for it, so that the last line of the file is the launch that faulted
-        with open(_DEBUG_SYNC, "a") as f:
-            f.write(what + "\n")
-        torch.cuda.synchronize()
+        _debug_sync(what)
     if rc != 0:
         msg = lib().rsdf_last_error()
         raise RiseSdfHipError(f"{what} failed (code {rc}): {msg.decode() if msg else ''}")
@@ -349,7 +354,29 @@ def nodes():
                 ("last_error", "embedding_fwd", "embedding_bwd_workspace_bytes", "embedding_bwd", "class_head_workspace_bytes",
                  "class_head_fwd", "class_head_bwd")], RiseSdfHipError)
         _nodes = m
+        _watch_nodes()
     return _nodes
+
+
+def _watch(name, args):
+    """What ``_TimedLib`` and ``check`` do around an entry point, for the C++ nodes: called before it; the result is called behind it."""
+    timer = _timer
+    if timer is not None:
+        e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        e0.record()
+
+    def done():
+        if timer is not None:
+            e1.record()
+            timer.records.append(("rsdf_" + name, args, e0, e1))
+        if _DEBUG_SYNC:
+            _debug_sync(name)
+    return done
+
+
+def _watch_nodes():
+    if _nodes is not None:
+        _nodes.watch(_watch if _timer is not None or _DEBUG_SYNC else None)
 
 
 # ---- transient workspaces -----------------------------------------------------------------------------------------------

@@ -11,6 +11,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
+#include <atomic>
 #include <unordered_set>
 
 namespace {
@@ -40,6 +41,28 @@ void check(int rc, const char *what)
     if (rc == 0) return;
     const char *msg = E.last_error();
     throw Error(std::string(what) + " failed (code " + std::to_string(rc) + "): " + (msg != nullptr ? msg : ""));
+}
+
+// Timers and the debug log of the Python layer (_lib._watch): called before each entry point with its name and scalar arguments; what it
+// returns is called behind it.
+std::atomic<bool> watched{false};
+py::object *watcher = nullptr;             // (only touched with the interpreter's lock; kept for the life of the process)
+
+template <class F, class... A> void entry(const char *name, F call, A... scalars)
+{
+    if (!watched.load(std::memory_order_relaxed)) {
+        check(call(), name);
+        return;
+    }
+    py::gil_scoped_acquire lock;
+    const py::object done = watched.load() ? (*watcher)(name, py::make_tuple(scalars...)) : py::none();
+    int rc;
+    {
+        py::gil_scoped_release free;
+        rc = call();
+    }
+    if (!done.is_none()) done();
+    check(rc, name);
 }
 
 int dtype_id(const Tensor &t)
@@ -117,9 +140,10 @@ struct Embedding : torch::autograd::Function<Embedding> {
         auto shape = ids.sizes().vec();
         shape.push_back(d);
         Tensor out = at::empty(shape, table.options().requires_grad(false));
-        check(E.embedding_fwd(address<const int64_t>(ids), ids.numel(), address<const void>(table), v, (int)d, dtype_id(table), (float)scale,
-                              padding, address<void>(out), (int32_t *)bad_ids, stream_of(table)),
-              "embedding_fwd");
+        entry("embedding_fwd", [&] {
+            return E.embedding_fwd(address<const int64_t>(ids), ids.numel(), address<const void>(table), v, (int)d, dtype_id(table), (float)scale,
+                                   padding, address<void>(out), (int32_t *)bad_ids, stream_of(table));
+        }, ids.numel(), v, d, dtype_id(table));
         ctx->save_for_backward({ids});
         ctx->saved_data["v"] = v;
         ctx->saved_data["d"] = d;
@@ -138,10 +162,11 @@ struct Embedding : torch::autograd::Function<Embedding> {
         Tensor dt = at::empty({v, d}, g.options());
         const int64_t bytes = E.embedding_bwd_workspace_bytes(n, v, (int)d);
         const Tensor ws = bytes > 0 ? bytes_on(bytes, g) : Tensor();
-        check(E.embedding_bwd(address<const int64_t>(ids), n, address<const void>(g), v, (int)d, dtype_id(g),
-                              (float)ctx->saved_data["scale"].toDouble(), ctx->saved_data["padding"].toInt(), address<void>(dt),
-                              address<void>(ws), bytes, stream_of(g)),
-              "embedding_bwd");
+        entry("embedding_bwd", [&] {
+            return E.embedding_bwd(address<const int64_t>(ids), n, address<const void>(g), v, (int)d, dtype_id(g),
+                                   (float)ctx->saved_data["scale"].toDouble(), ctx->saved_data["padding"].toInt(), address<void>(dt),
+                                   address<void>(ws), bytes, stream_of(g));
+        }, n, v, d, dtype_id(g));
         return once({Tensor(), dt, Tensor(), Tensor(), Tensor()}, "embedding");
     }
 };
@@ -170,11 +195,12 @@ struct ClassHead : torch::autograd::Function<ClassHead> {
         const Tensor keep = at::empty({2 * n + 1 + (teacher ? 2 * n * k : 0)}, f32);
         Tensor loss = reduction == 0 ? at::empty({n}, f32) : at::empty({}, f32);
         float *a = address<float>(keep), *q = teacher ? a + 2 * n + 1 : nullptr;
-        check(E.class_head_fwd(address<const void>(x), address<const void>(w), n, v, (int)d, dtype_id(x), address<const int64_t>(ids),
-                               teacher ? address<const float>(*logits) : nullptr, (int)k, ignore, (float)temperature, (int)reduction,
-                               address<float>(loss), a, a + 2 * n, q, teacher ? q + n * k : nullptr, (int32_t *)bad_ids, address<void>(ws), bytes,
-                               stream_of(x)),
-              "class_head_fwd");
+        entry("class_head_fwd", [&] {
+            return E.class_head_fwd(address<const void>(x), address<const void>(w), n, v, (int)d, dtype_id(x), address<const int64_t>(ids),
+                                    teacher ? address<const float>(*logits) : nullptr, (int)k, ignore, (float)temperature, (int)reduction,
+                                    address<float>(loss), a, a + 2 * n, q, teacher ? q + n * k : nullptr, (int32_t *)bad_ids,
+                                    address<void>(ws), bytes, stream_of(x));
+        }, n, v, d, dtype_id(x), k);
         ctx->save_for_backward({x, w, ids, keep});
         ctx->saved_data["k"] = k;
         ctx->saved_data["temperature"] = temperature;
@@ -200,11 +226,12 @@ struct ClassHead : torch::autograd::Function<ClassHead> {
         const int64_t bytes = E.class_head_workspace_bytes(n, v, (int)d, dtype_id(x), (need_x ? 1 : 0) + (need_w ? 2 : 0));
         const Tensor ws = bytes_on(bytes, x);
         float *a = address<float>(keep), *q = teacher ? a + 2 * n + 1 : nullptr;
-        check(E.class_head_bwd(address<const void>(x), address<const void>(w), n, v, (int)d, dtype_id(x), address<const int64_t>(ids), q,
-                               teacher ? q + n * k : nullptr, (int)k, (float)ctx->saved_data["temperature"].toDouble(), a,
-                               reduction == 1 ? a + 2 * n : nullptr, address<const float>(g), reduction == 0, address<void>(out[0]),
-                               address<void>(out[1]), address<void>(ws), bytes, stream_of(x)),
-              "class_head_bwd");
+        entry("class_head_bwd", [&] {
+            return E.class_head_bwd(address<const void>(x), address<const void>(w), n, v, (int)d, dtype_id(x), address<const int64_t>(ids), q,
+                                    teacher ? q + n * k : nullptr, (int)k, (float)ctx->saved_data["temperature"].toDouble(), a,
+                                    reduction == 1 ? a + 2 * n : nullptr, address<const float>(g), reduction == 0, address<void>(out[0]),
+                                    address<void>(out[1]), address<void>(ws), bytes, stream_of(x));
+        }, n, v, d, dtype_id(x), k);
         return once(std::move(out), "the losses of a linear head");
     }
 };
@@ -236,6 +263,12 @@ void bind(const std::vector<uintptr_t> &a, py::object error)
 PYBIND11_MODULE(_codebook, m)
 {
     m.def("bind", &bind);
+    m.def("watch", [](py::object call) {
+        watched = false;
+        if (watcher == nullptr) watcher = new py::object();
+        *watcher = call;
+        watched = !call.is_none();
+    });
     m.def("embedding", [](const Tensor &ids, const Tensor &table, double scale, int64_t padding, int64_t bad_ids) {
         py::gil_scoped_release free;
         check_leaves(table, "embedding");
