@@ -736,6 +736,10 @@ int rsdf_embedding_bwd(const int64_t *ids, int64_t n, const void *grad, int64_t 
  * workspace: >= rsdf_class_head_workspace_bytes(n, v, d, dtype, pass), pass 0 forward, else backward (1 dx, 2 dw, 3 both): the
  * forward's holds 8 bytes per row and 256 (few tiles: 128) classes, the backward's one piece of the classes, 128 MB or 256 classes. */
 int64_t rsdf_class_head_workspace_bytes(int64_t n, int64_t v, int d, int dtype, int pass);
+/* How a head of these sizes is computed (host only): plan[8] = rows of z's forward tile (32, 128 or 256), of its backward tile (128 or
+ * 256), of the products' tile (128 or 256); pieces of the classes, forward and backward; cuts over k of dw and of dx; 1 if the operands
+ * are read where they are (0: packed first). */
+int rsdf_class_head_plan(int64_t n, int64_t v, int d, int dtype, int32_t *plan);
 int rsdf_class_head_fwd(const void *x, const void *w, int64_t n, int64_t v, int d, int dtype, const int64_t *ids,
                         const float *teacher_logits /*nullable*/, int k, int64_t ignore_id, float temperature, int reduction,
                         float *loss, float *lse, float *count, float *q, float *listed_z, int32_t *bad_ids,

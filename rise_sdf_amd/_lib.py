@@ -169,6 +169,7 @@ _SIGNATURES = {
     "rsdf_embedding_bwd_workspace_bytes": [_L, _L, _I],
     "rsdf_embedding_bwd": [_P, _L, _P, _L, _I, _I, _F, _L, _P, _P, _L, _P],
     "rsdf_class_head_workspace_bytes": [_L, _L, _I, _I, _I],
+    "rsdf_class_head_plan": [_L, _L, _I, _I, _P],
     "rsdf_class_head_fwd": [_P, _P, _L, _L, _I, _I, _P, _P, _I, _L, _F, _I, _P, _P, _P, _P, _P, _P, _P, _L, _P],
     "rsdf_class_head_bwd": [_P, _P, _L, _L, _I, _I, _P, _P, _P, _I, _F, _P, _P, _P, _I, _P, _P, _P, _L, _P],
 }
@@ -267,7 +268,7 @@ class _TimedLib:
         fn = getattr(self._l, name)
         # host-only queries launch nothing: not timed
         if not name.startswith("rsdf_") or "_supported" in name or name.endswith(("_scratch_bytes", "_workspace_bytes")) or \
-                name in ("rsdf_last_error", "rsdf_abi_version", "rsdf_grid_meta_init"):
+                name in ("rsdf_last_error", "rsdf_abi_version", "rsdf_grid_meta_init", "rsdf_class_head_plan"):
             return fn
         timer = self._t
 

@@ -1161,6 +1161,18 @@ int64_t rsdf_class_head_workspace_bytes(int64_t n, int64_t v, int d, int dtype, 
     return s.at;
 }
 
+int rsdf_class_head_plan(int64_t n, int64_t v, int d, int dtype, int32_t *plan)
+{
+    const char *bad = bad_head(n, v, d, dtype, 1, nullptr, nullptr);
+    RSDF_CHECK_ARG(bad == nullptr, bad);
+    RSDF_CHECK_ARG(plan != nullptr, "class_head_plan: plan must not be NULL");
+    const Plan p = make_plan(n, v, d, dtype);
+    const int32_t out[8] = {p.small ? 32 : (p.quarter_fwd ? 128 : 256), p.quarter_bwd ? 128 : 256, p.bm,
+                            (int32_t)((v + p.vf - 1) / p.vf), (int32_t)((v + p.vc - 1) / p.vc), p.split_dw, p.split_dx, p.direct};
+    for (int i = 0; i < 8; ++i) plan[i] = out[i];
+    return 0;
+}
+
 int rsdf_class_head_fwd(const void *x, const void *w, int64_t n, int64_t v, int d, int dtype, const int64_t *ids,
                         const float *teacher_logits, int k, int64_t ignore_id, float temperature, int reduction, float *loss,
                         float *lse, float *count, float *q, float *listed_z, int32_t *bad_ids, void *workspace,
