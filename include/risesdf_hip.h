@@ -733,8 +733,12 @@ int rsdf_embedding_bwd(const int64_t *ids, int64_t n, const void *grad, int64_t 
  *   of the first listed class), q [n][k] and listed_z [n][k] (teacher only) are what bwd reads.
  * bwd: grad = d(loss): [n] (grad_per_row) or [1]; count as written by fwd for reduction 1, else NULL.  dx [n][d] / dw [v][d]
  *   (nullable: not computed).
- * workspace: >= rsdf_class_head_workspace_bytes(n, v, d, dtype, pass), pass 0 forward, else backward (1 dx, 2 dw, 3 both): the
- * forward's holds 8 bytes per row and 256 (few tiles: 128) classes, the backward's one piece of the classes, 128 MB or 256 classes. */
+ * workspace: >= rsdf_class_head_workspace_bytes(n, v, d, dtype, pass), pass 0 forward, else backward (1 dx, 2 dw, 3 both).  With n' = n
+ * and d' = d rounded up to 256 and 64, s = 2 bytes (fp32: 6):
+ *   forward   8 bytes per row and 256 (few tiles: 128) classes; unless d % 8 == 0 in 16 bits also x, n' d' s, and at most 128 MB (or 256 rows)
+ *             of w
+ *   backward  one piece of dz, at most 128 MB or 256 classes, 256 n' s (more than 128 MB beyond 2^18 rows, fp32: 87381); x as above; w of the
+ *             piece; 32-bit partial sums of dx, up to 64 n d' (few where rows are many), and of dw, up to 64 times the piece's d' */
 int64_t rsdf_class_head_workspace_bytes(int64_t n, int64_t v, int d, int dtype, int pass);
 /* How a head of these sizes is computed (host only): plan[8] = rows of z's forward tile (32, 128 or 256), of its backward tile (128 or
  * 256), of the products' tile (128 or 256); pieces of the classes, forward and backward; cuts over k of dw and of dx; 1 if the operands

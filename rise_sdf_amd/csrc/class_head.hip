@@ -13,8 +13,8 @@
 // the tiles' sums and joined from its dot product: with R the sum over the others, lse - z_y = log(1 + R exp(-z_y)) and
 // 1 - p_y = 1 / (1 + exp(z_y) / R) keep all their digits where the head is sure of itself, and both uses of z_y see one rounding.
 // Backward, in pieces of the classes: the tiles are computed again and leave as 16-bit dz [rows][piece]; two products read it
-// (dx over the piece, dw of the piece).  A piece is at most DZ_BYTES: it is still in the last-level cache when it is read
-// (products at V = 131072: 1005 us; with 64 MB pieces, twice as many launches, 1267, with 256 MB 1273).
+// (dx over the piece, dw of the piece).  A piece is at most DZ_BYTES, unless 256 classes of all the rows are more (beyond 2^18 rows, fp32 87381):
+// it is still in the last-level cache when it is read (products at V = 131072: 1005 us; with 64 MB pieces, twice as many launches, 1267, with 256 MB 1273).
 //
 // Bound by the matrix units, and by what runs between products.  4096 x 32768 x 512 bf16: z 152 us (0.90 PF/s, about a quarter of
 // it the exponentials), dz 174, the two products 275 (1.0 PF/s); matrix units busy half the cycles at 1.7-1.8 GHz.  32 rows or less are

@@ -31,3 +31,26 @@ def test_plan_refusals():
     for size in ((0, 8, 8, 0), (4, 0, 8, 0), (4, 8, 0, 0), (4, 8, 8, 3)):
         assert lib.rsdf_class_head_plan(*size, out) == 10001
     assert lib.rsdf_class_head_plan(4, 8, 8, 0, None) == 10001
+
+
+@pytest.mark.parametrize("n,v,d", [(4096, 131072, 512), (4096, 32768, 512), (8192, 131072, 64), (256, 1 << 22, 64), (65536, 65536, 512), (1 << 18, 8192, 64),
+                                   (1 << 20, 1000, 48), (1 << 24, 256, 64), (1, 53163, 697), (4096, 1000, 48)])
+@pytest.mark.parametrize("kind", [0, 1, 2])
+def test_workspace_is_the_sum_of_its_stated_terms(n, v, d, kind):
+    size = _lib.lib().rsdf_class_head_workspace_bytes
+    p, s = plan(n, v, d, kind), 6 if kind == 0 else 2
+    rows, dp = -(-n // 256) * 256, -(-d // 64) * 64
+    packed, mb = not p["direct"], 1 << 20
+    x, w = rows * dp * s, max(128 * mb, 256 * dp * s)
+    forward = 8 * n * -(-v // 128) + 4 * n + packed * (x + w) + 2048
+    assert int(size(n, v, d, kind, 0)) <= forward
+    piece = max(128 * mb, 256 * rows * s)
+    classes = piece // (rows * s)
+    dx = 4 * p["split_dx"] * n * dp
+    dw = 4 * p["split_dw"] * classes * dp if p["split_dw"] > 1 else 0
+    for which in (1, 2, 3):
+        bound = piece + x + packed * w + (which & 1) * dx + (which >> 1) * dw + 4 * n + 2048
+        assert int(size(n, v, d, kind, which)) <= bound
+    # no logits: where they would be much, the backward's space is a part of them alone in 16 bits
+    if n * v * 2 >= 1 << 30 and n <= 1 << 16:
+        assert int(size(n, v, d, kind, 3)) < n * v * 2 // 4
