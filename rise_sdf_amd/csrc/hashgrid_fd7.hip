@@ -467,20 +467,11 @@ __device__ __forceinline__ void x2_store_points(const X2Out &o, const TapSrc &sr
 #ifndef RSDF_BWD_GROUP
 #define RSDF_BWD_GROUP 64      // producer: 64 x 1024 samples (0.8 MB of centres) per group: the 15 re-reads of a group's centres hit
 #endif                         // in the XCD's L2 (256: they come back from the MALL, +150 B per sample of fetch traffic; same time)
-using pk_f32x2 = __attribute__((ext_vector_type(2))) float;
-// acc += w v on both features: the same two fmas, written as a packed one (this file is built with -fno-slp-vectorize:
-// packed fp32 arithmetic that the compiler forms by itself costs more than it saves on gfx950 -- producer 21.8 -> 21.4 ms
-// without it -- but the gather's accumulation is faster packed: 12.26 vs 12.40 ms)
+// acc += w v on both features (packed fp32 arithmetic, off in every unit, was 1 % faster here and nowhere else: 12.26 and 12.40 ms)
 __device__ __forceinline__ void fma2(float2 &acc, float w, const float2 &v)
 {
-#ifdef RSDF_FWD_SCALAR_FMA
     acc.x = fmaf(w, v.x, acc.x);
     acc.y = fmaf(w, v.y, acc.y);
-#else
-    const pk_f32x2 r = __builtin_elementwise_fma(pk_f32x2{w, w}, pk_f32x2{v.x, v.y}, pk_f32x2{acc.x, acc.y});
-    acc.x = r[0];
-    acc.y = r[1];
-#endif
 }
 
 template <bool DERIVE, bool X3>
@@ -631,19 +622,6 @@ struct StamperP {
 };
 #define RSDF_PSTAMP(st, i)
 #endif
-
-// a += w g, one fma per feature
-__device__ __forceinline__ void axpy2(float2 &a, float w, pk_f32x2 g)
-{
-#ifndef RSDF_AXPY_PACKED      // (as a packed fma the producer needs 54 spilled registers instead of 13: 23.9 vs 21.4 ms)
-    a.x = fmaf(w, g[0], a.x);
-    a.y = fmaf(w, g[1], a.y);
-#else
-    const pk_f32x2 r = __builtin_elementwise_fma(pk_f32x2{w, w}, g, pk_f32x2{a.x, a.y});
-    a.x = r[0];
-    a.y = r[1];
-#endif
-}
 
 // d_planes are read once per launch by phase 1 (the displaced taps of phase 2 re-read a few of them from L2)
 __device__ __forceinline__ float2 ld_dplane(const float2 *p)
@@ -853,23 +831,23 @@ fd7_produce_kernel(const TapSrc src, const float2 *__restrict__ dplanes,
                 const int t = 2 * a + 1 + sd;
                 const CellFrac ct = cf[t];
                 const float2 gr = ld_dplane(pg + (int64_t)t * S);
-                const pk_f32x2 g2 = {gr.x, gr.y};
+                const float2 g2 = make_float2(gr.x, gr.y);
                 const int32_t da = (int32_t)(ct.c[a] - c0.c[a]);
                 const float wa[2] = {1.0f - ct.w[a], ct.w[a]};
                 if (da == 0) {
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
 #pragma unroll
-                        for (int b = 0; b < 2; ++b) axpy2(acc[(b << a) | ((k & 1) << o1) | ((k >> 1) << o2)], oth[k] * wa[b], g2);
+                        for (int b = 0; b < 2; ++b) fma2(acc[(b << a) | ((k & 1) << o1) | ((k >> 1) << o2)], oth[k] * wa[b], g2);
                 } else if (da == 1) {
                     // the tap's near face (its corners with bit a == 0) coincides with the centre cell's far face (bit a == 1)
                     items |= 3u << (2 * (t - 1));
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) axpy2(acc[(1 << a) | ((k & 1) << o1) | ((k >> 1) << o2)], oth[k] * wa[0], g2);
+                    for (int k = 0; k < 4; ++k) fma2(acc[(1 << a) | ((k & 1) << o1) | ((k >> 1) << o2)], oth[k] * wa[0], g2);
                 } else if (da == -1) {
                     items |= 1u << (2 * (t - 1));
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) axpy2(acc[((k & 1) << o1) | ((k >> 1) << o2)], oth[k] * wa[1], g2);
+                    for (int k = 0; k < 4; ++k) fma2(acc[((k & 1) << o1) | ((k >> 1) << o2)], oth[k] * wa[1], g2);
                 } else {  // tap more than one cell away (eps larger than a cell): rare slow path
 #pragma unroll
                     for (int c = 0; c < 8; ++c) {

@@ -6,8 +6,8 @@ set -euo pipefail
 : "${GRAFT_REPO_ROOT:?run on the GPU box through gpurun (sets GRAFT_REPO_ROOT)}"
 cd "$GRAFT_REPO_ROOT/rise_sdf_amd/csrc"
 mkdir -p /tmp/ab_all
-F="-O3 -std=c++17 --offload-arch=gfx950 -ffp-contract=off -fPIC -w $1"
-for s in core march composite hashgrid hashgrid_fd7 hashgrid_dx mlp mlp_fused mlp_coop mlp_quad mlp_x2 mlp_pair mlp_layer_bwd neus texture gridsample envlight frontend loss; do
+F="-O3 -std=c++17 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -ffp-contract=off -fPIC -w $1"
+for s in core march composite hashgrid hashgrid_fd7 hashgrid_dx mlp mlp_fused mlp_coop mlp_quad mlp_x2 mlp_pair mlp_layer_bwd neus texture gridsample envlight frontend loss class_head embedding; do
   /opt/rocm/bin/hipcc $F -c $s.hip -o /tmp/ab_all/$s.o &
 done
 for s in mlp mlp_fused mlp_coop mlp_quad mlp_layer_bwd; do

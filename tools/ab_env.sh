@@ -9,7 +9,7 @@ mkdir -p /tmp/ab; rm -f /tmp/ab/*.o
 export RSDF_LIB=/tmp/ab/librisesdf_hip.variant.so
 variant_objs() { for o in _build/*.o; do b=$(basename $o); if [ -f /tmp/ab/$b ]; then echo /tmp/ab/$b; else echo $o; fi; done; }
 for v in "$@"; do
-  /opt/rocm/bin/hipcc -O3 -std=c++17 --offload-arch=gfx950 -ffp-contract=off -fPIC -I../../include $v -c envlight.hip -o /tmp/ab/envlight.o
+  /opt/rocm/bin/hipcc -O3 -std=c++17 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -ffp-contract=off -fPIC -I../../include $v -c envlight.hip -o /tmp/ab/envlight.o
   /opt/rocm/bin/hipcc -shared -fPIC --offload-arch=gfx950 $(variant_objs) -o $RSDF_LIB
   (cd ../.. && bash tools/spec_levels.sh | head -6 | awk '{print $(NF-1)}' | tr '\n' ' '; echo " <= [$v]")
 done

@@ -11,7 +11,7 @@ export RSDF_LIB=/tmp/ab/librisesdf_hip.variant.so
 variant_objs() { for o in _build/*.o; do b=$(basename $o); if [ -f /tmp/ab/$b ]; then echo /tmp/ab/$b; else echo $o; fi; done; }
 for v in "$@"; do
   for f in mlp_fused mlp_coop mlp_quad; do
-    /opt/rocm/bin/hipcc -O3 -std=c++17 --offload-arch=gfx950 -ffp-contract=off -fPIC -I../../include $v -c $f.hip -o /tmp/ab/$f.o
+    /opt/rocm/bin/hipcc -O3 -std=c++17 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -ffp-contract=off -fPIC -I../../include $v -c $f.hip -o /tmp/ab/$f.o
   done
   /opt/rocm/bin/hipcc -shared -fPIC --offload-arch=gfx950 $(variant_objs) -o $RSDF_LIB
   for h in 64 128; do

@@ -1,7 +1,7 @@
 // Is a 16-byte gather of an aligned entry pair as cheap as ONE 8-byte gather?  (hash-grid corner pairs along x)
 // Random entries of a 4 MiB table (one hashed level), 64 independent gathers in flight per lane.
 //   mode 0: two float2 loads (idx, idx ^ 1)      mode 1: one float4 load (idx & ~1)      mode 2: one float2 load
-// Build: hipcc -O2 --offload-arch=gfx950 tools/gather_pair_bench.hip -o tools/_build/gather_pair_bench
+// Build: hipcc -O2 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops tools/gather_pair_bench.hip -o tools/_build/gather_pair_bench
 #include <hip/hip_runtime.h>
 #include <cstdio>
 __global__ void k(const float2 *__restrict__ t, int mode, unsigned mask, int iters, float *out)

@@ -1,5 +1,5 @@
 // Micro-benchmark: LDS atomic throughput on gfx950 for random addresses (run on the GPU box).
-//   hipcc --offload-arch=gfx950 -O3 tools/lds_atomic_bench.hip -o /tmp/lds_bench && /tmp/lds_bench
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 tools/lds_atomic_bench.hip -o /tmp/lds_bench && /tmp/lds_bench
 #include <hip/hip_runtime.h>
 #include <stdio.h>
 #include <stdint.h>

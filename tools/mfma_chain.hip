@@ -1,6 +1,6 @@
 // Issue-to-issue cost of DEPENDENT bf16 MFMAs on gfx950: C chains of v_mfma_f32_32x32x16_bf16 (or 16x16x32), each
 // instruction accumulating into the previous result of its chain.  Prints cycles per MFMA for C = 1, 2, 4.
-// Build: hipcc -O2 --offload-arch=gfx950 tools/mfma_chain.hip -o tools/_build/mfma_chain
+// Build: hipcc -O2 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops tools/mfma_chain.hip -o tools/_build/mfma_chain
 #include <hip/hip_runtime.h>
 #include <cstdio>
 using f32x16 = __attribute__((ext_vector_type(16))) float;

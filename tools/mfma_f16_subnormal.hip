@@ -1,6 +1,6 @@
 // Does v_mfma_f32_32x32x16_f16 / 16x16x32_f16 keep fp16 SUBNORMAL inputs (needed by the two-part fp16 split of fp32 operands:
 // the low part of a value near the bottom of the fp16 range is subnormal)?  Also times f16 against bf16 MFMAs.
-//   hipcc --offload-arch=gfx950 -O3 tools/mfma_f16_subnormal.hip -o tools/_build/mfma_f16_subnormal && tools/_build/mfma_f16_subnormal
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 tools/mfma_f16_subnormal.hip -o tools/_build/mfma_f16_subnormal && tools/_build/mfma_f16_subnormal
 #include <hip/hip_runtime.h>
 #include <cstdio>
 using f32x16 = __attribute__((ext_vector_type(16))) float;

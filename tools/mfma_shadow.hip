@@ -1,7 +1,7 @@
 // How many vector-ALU instructions fit in the shadow of one bf16 MFMA on gfx950?  Exact instruction streams (inline asm):
 // per loop step 4 x { v_mfma_f32_32x32x16_bf16 (or 2 x 16x16x32); K x v_fma_f32 }, two independent accumulator chains.
 // Prints s_memtime cycles per MFMA for K = 0..12, with one and with two waves per SIMD, and for v_exp_f32 fillers.
-// Build: hipcc -O2 --offload-arch=gfx950 tools/mfma_shadow.hip -o tools/_build/mfma_shadow
+// Build: hipcc -O2 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops tools/mfma_shadow.hip -o tools/_build/mfma_shadow
 #include <hip/hip_runtime.h>
 #include <cstdio>
 using f32x16 = __attribute__((ext_vector_type(16))) float;

@@ -5,7 +5,7 @@
 //   4: like 3 but waves 4-7 start with the VALU burst (out of phase)
 //   5: every wave: MFMA and VALU finely interleaved (1 MFMA : M/N VALU)
 // Prints wall microseconds per mode; shape s = 0: 32x32x2, 1: 16x16x4.
-// Build: hipcc -O2 --offload-arch=gfx950 tools/mfma_valu_overlap.hip -o tools/_build/mfma_valu_overlap
+// Build: hipcc -O2 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops tools/mfma_valu_overlap.hip -o tools/_build/mfma_valu_overlap
 #include <hip/hip_runtime.h>
 #include <cstdio>
 using f32x16 = __attribute__((ext_vector_type(16))) float;

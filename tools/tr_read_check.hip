@@ -1,7 +1,7 @@
 // Checks on the box (a) the lane <-> element map of ds_read_b64_tr_b16 as cdna_hip_programming.md T10 states it and
 // (b) that two tr-read fragments of [row][feature] bf16 images feed v_mfma_f32_32x32x16_bf16 as
 // C[i][j] = sum_r P[r][i] Q[r][j]  (the weight-gradient product of mlp_coop.hip: rows are the MFMA k dimension).
-//   hipcc --offload-arch=gfx950 -O3 tools/tr_read_check.hip -o tools/_build/tr_read_check && tools/_build/tr_read_check
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 tools/tr_read_check.hip -o tools/_build/tr_read_check && tools/_build/tr_read_check
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdlib>

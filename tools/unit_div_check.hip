@@ -1,7 +1,7 @@
 // Exhaustive check of hashgrid_common.h's unit_div (five multiply-adds) against the IEEE division it replaces: all 2^32 bit
 // patterns of x for each divisor of a list (2 r of the yamls' radius 1.5 first), the quotients compared bit for bit.
 // (models/geometry.py:229-244's contraction (q - (-r)) / (r - (-r)), which neus.hip fd_points_kernel performs as a division.)
-//   hipcc -O3 --offload-arch=gfx950 -ffp-contract=off -I rise_sdf_amd/csrc -I include -o /tmp/unit_div_check tools/unit_div_check.hip
+//   hipcc -O3 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -ffp-contract=off -I rise_sdf_amd/csrc -I include -o /tmp/unit_div_check tools/unit_div_check.hip
 //   /tmp/unit_div_check
 // Prints, per divisor: mismatches among the x the fast path is specified for (x == +0 or 2^-100 < |x| < 2^100) and among the
 // rest (-0, tiny, huge, non-finite: documented as out of contract).  Exit code 1 if any in-contract quotient differs.

@@ -1,5 +1,5 @@
 // Which SIMD does wave w of a workgroup land on?  (HW_REG_HW_ID: SIMD_ID bits [5:4], CU_ID [11:8] on gfx9-family.)
-// Build: hipcc -O2 --offload-arch=gfx950 tools/wave_simd_map.hip -o tools/_build/wave_simd_map
+// Build: hipcc -O2 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops tools/wave_simd_map.hip -o tools/_build/wave_simd_map
 #include <hip/hip_runtime.h>
 #include <cstdio>
 __global__ void probe(int *out)
