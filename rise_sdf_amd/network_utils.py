@@ -106,6 +106,8 @@ class EmbeddingEncoding(nn.Module):
         self.n_output_dims = int(config["n_features"])
         self.scale = float(config.get("scale", 1.0))
         self.padding_idx = config.get("padding_idx", None)
+        if self.padding_idx is not None and not 0 <= int(self.padding_idx) < int(config["n_embeddings"]):
+            raise ValueError(f"Embedding: padding_idx {self.padding_idx} outside its {config['n_embeddings']} codes")
         self.params = nn.Parameter(torch.randn(int(config["n_embeddings"]), self.n_output_dims) * float(config.get("std", 0.01)))
         if self.padding_idx is not None:
             with torch.no_grad():
