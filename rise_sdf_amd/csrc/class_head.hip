@@ -17,7 +17,7 @@
 // it is still in the last-level cache when it is read (products at V = 131072: 1005 us; with 64 MB pieces, twice as many launches, 1267, with 256 MB 1273).
 //
 // Bound by the matrix units, and by what runs between products.  4096 x 32768 x 512 bf16: z 152 us (0.90 PF/s, about a quarter of
-// it the exponentials), dz 174, the two products 275 (1.0 PF/s); matrix units busy half the cycles at 1.7-1.8 GHz.  32 rows or less are
+// it the exponentials), dz 174, the two products 275 (1.0 PF/s); matrix units busy 43, 36 and 48 % of the cycles, at 1.7-1.8 GHz.  32 rows or less are
 // bound by reading the codes: 16 x 65536 x 512 bf16 13.7 us (4.9 TB/s).
 //
 // Number formats.  bf16 and fp16 operands enter the matrix unit as they are, sums are fp32.  fp32 operands are split into three
@@ -380,7 +380,7 @@ __device__ __forceinline__ void head_results(const HeadArgs &a, typename TL::Acc
                     for (int e = 0; e < 16; ++e) p[e] = -p[e];
                 }
                 if (label >= 0 && label < 16) {
-                    const float miss = a.lse[a.n + n0 + TL::n_of(nt)];
+                    const float miss = a.lse[a.n + n0 + TL::n_of(nt)];      // (in a walk this waits for the next tile's requests too)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) p[e] = e == label ? -miss * f : p[e];
                 }
